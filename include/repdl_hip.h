@@ -10,7 +10,8 @@
  *
  * Conventions
  *   - All pointers are DEVICE pointers to contiguous row-major float32 data
- *     (int64 for class labels) on the device that is current when the call is
+ *     (int64 for class labels; the operators that take a `dtype` also 16-bit
+ *     types, see REPDL_BF16) on the device that is current when the call is
  *     made.  Outputs are caller-allocated.  Inputs are never written
  *     (the optimizer steps update their state tensors in place and say so).
  *   - `stream` is a hipStream_t passed as void* (NULL = the default stream).
@@ -115,6 +116,13 @@ int repdl_hip_init(void);
 int repdl_hip_mfma_selftest(int64_t waves, int64_t trials, uint64_t seed, uint64_t *mismatches);
 int repdl_hip_set_matrix_path(int mode);
 int repdl_hip_matrix_path(void);
+
+/* Element types of the operators that take more than binary32 (layer_norm, dropout, preference_loss; every other
+ * entry point is binary32).  They compute in binary32 whatever the type: elements are widened exactly when they are
+ * read and rounded once, to nearest even, when they are written. */
+#define REPDL_F32 0
+#define REPDL_BF16 1
+#define REPDL_F16 2
 
 /* mm -- backend/cuda/matrix_multiplication.cu:234-260 (bound at :267);
  * semantics backend/cpu/matrix_multiplication.cpp:12-36.
@@ -293,6 +301,70 @@ int repdl_hip_bn_gvar_term(const float *grad_y, const float *x, const float *mea
                            int64_t outer, int64_t channels, int64_t inner, void *stream);
 int repdl_hip_bn_gweight_term(const float *x, const float *mean, const float *std, const float *grad_y, float *out,
                               int64_t outer, int64_t channels, int64_t inner, void *stream);
+
+/* Layer normalisation.  No counterpart in the reference (its only normalisation is the batch norm above).  x and y are
+ * [M,N] of `dtype`, weight and bias [N] of `param_dtype` (either may be NULL: no such factor, no such term), param_dtype is
+ * dtype or REPDL_F32; mean and rstd are [M] binary32, for the backward pass (both NULL: not wanted).  Per row:
+ *   mean = S(x_j) * float(1/N),  var = S(RN(d_j * d_j)) * float(1/N) with d_j = RN(x_j - mean),
+ *   rstd = RN(1 / RN(sqrt(RN(var + eps)))),  y_j = RN(RN(RN(d_j * rstd) * weight_j) + bias_j)
+ * S is a binary32 sum whose order N and the type determine alone: the same row gives the same bits whatever the other
+ * rows, the addresses, the stream and the device.
+ * Backward, with xh_j = RN(d_j * rstd) and g_j = RN(grad_y_j * weight_j):
+ *   grad_x_j    = RN(rstd * RN(RN(g_j - c1) - RN(xh_j * c2))),  c1 = S(g_j) * float(1/N),  c2 = S(RN(g_j * xh_j)) * float(1/N)
+ *   grad_weight = S over the rows of RN(grad_y_ij * xh_ij),  grad_bias = S over the rows of grad_y_ij
+ * (the order of the sums over rows is a function of M, N and the type; they are rounded to param_dtype at the end).  Any of
+ * grad_x, grad_weight, grad_bias may be NULL: not wanted.  M = 0 gives zeros in grad_weight and grad_bias.
+ * Scratch (see "Scratch memory"): at most 512 rows of 2 N floats for the two sums over rows. */
+int repdl_hip_layer_norm(const void *x, const void *weight, const void *bias, void *y, float *mean, float *rstd, int64_t M,
+                         int64_t N, float eps, int dtype, int param_dtype, void *stream);
+int repdl_hip_layer_norm_grad(const void *grad_y, const void *x, const void *weight, const float *mean, const float *rstd,
+                              void *grad_x, void *grad_weight, void *grad_bias, int64_t M, int64_t N, int dtype,
+                              int param_dtype, void *stream);
+size_t repdl_hip_layer_norm_grad_workspace_bytes(int64_t M, int64_t N);
+int repdl_hip_layer_norm_grad_ws(const void *grad_y, const void *x, const void *weight, const float *mean,
+                                 const float *rstd, void *grad_x, void *grad_weight, void *grad_bias, int64_t M, int64_t N,
+                                 int dtype, int param_dtype, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Dropout from a counter-based generator.  No counterpart in the reference.  Word j of the generator is word j % 4 of
+ * Philox4x32 with ten rounds (Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as easy as 1, 2, 3", 2011) for the key
+ * `seed` and the counter whose low 64 bits are j / 4 and whose high 64 bits are `call`: a function of (seed, call, j), the
+ * same on every device and for every type.  Element j is kept if its word >= round(p * 2^32) (p = 1: none is), and
+ *   y_j = RN(x_j * float(1 / (1 - p))) if kept, else +0;  with a residual y_j = RN(residual_j + that), else residual_j.
+ * The mask is not stored: the gradient with respect to x is the same call on the incoming gradient, without a residual.
+ * seed and call are read from DEVICE memory, state[0] and state[1], where `state` is not NULL (a graph's replays then follow
+ * what lies there), else they are the arguments.  repdl_hip_dropout_next_call: used = state, then state[1] += 1, both [2] on
+ * the device -- one call of a layer that keeps its own count.  Nothing is allocated. */
+int repdl_hip_dropout(const void *x, const void *residual, void *y, int64_t n, double p, const int64_t *state,
+                      uint64_t seed, uint64_t call, int dtype, void *stream);
+int repdl_hip_dropout_next_call(int64_t *state, int64_t *used, void *stream);
+
+/* Preference loss of paired answers from token logits.  No counterpart in the reference, whose loss is cross_entropy.
+ * logits: 2 * pairs sequences of `steps` rows of `vocab` contiguous elements of `dtype`; sequence i, step t starts at
+ * logits + i * seq_stride + t * step_stride (elements).  Sequence p < pairs is the preferred answer of pair p, sequence
+ * pairs + p the other one.  target is [2 * pairs, steps] int64, contiguous: the token that each row predicts, or ignore_index
+ * for a row that is not counted (prompt, padding) -- such a row's logits are not read.  ref_logps is [2 * pairs] binary32, the
+ * reference model's log probabilities of the sequences (NULL: zeros).  With lp = log softmax(row)[target] summed over a
+ * sequence's counted rows as L (binary64) and z_p = beta * ((L_p - L_{pairs+p}) - (ref_p - ref_{pairs+p})):
+ *   loss[0]  = mean over pairs of (1 - label_smoothing) * softplus(-z_p) + label_smoothing * softplus(z_p)
+ *   logps[i] = L_i, [2 * pairs]
+ * row_stats [2 * pairs, steps, 2] (8-byte aligned) and coef [2 * pairs] are what the backward pass takes (both NULL: not
+ * wanted).  A target outside [0, vocab) that is not ignore_index, a NaN or +inf logit and a row of nothing but -inf make their
+ * sequence's log probability, the loss and the pair's gradient NaN.
+ * preference_loss_grad: grad_logits [2 * pairs, steps, vocab], contiguous, = grad_loss[0] (device memory) * d loss / d logits;
+ * +0 on rows that are not counted.  The order of every sum is a function of the extents and the type alone.
+ * Scratch of the forward pass: 8 bytes per row and 16384 columns, 4 per row, 8 per pair. */
+int repdl_hip_preference_loss(const void *logits, const int64_t *target, const float *ref_logps, float *loss, float *logps,
+                              float *row_stats, float *coef, int64_t pairs, int64_t steps, int64_t vocab,
+                              int64_t seq_stride, int64_t step_stride, double beta, double label_smoothing,
+                              int64_t ignore_index, int dtype, void *stream);
+size_t repdl_hip_preference_loss_workspace_bytes(int64_t pairs, int64_t steps, int64_t vocab);
+int repdl_hip_preference_loss_ws(const void *logits, const int64_t *target, const float *ref_logps, float *loss,
+                                 float *logps, float *row_stats, float *coef, int64_t pairs, int64_t steps, int64_t vocab,
+                                 int64_t seq_stride, int64_t step_stride, double beta, double label_smoothing,
+                                 int64_t ignore_index, int dtype, void *workspace, size_t workspace_bytes, void *stream);
+int repdl_hip_preference_loss_grad(const void *logits, const int64_t *target, const float *row_stats, const float *coef,
+                                   const float *grad_loss, void *grad_logits, int64_t pairs, int64_t steps, int64_t vocab,
+                                   int64_t seq_stride, int64_t step_stride, int64_t ignore_index, int dtype, void *stream);
 
 /* Optimizer steps -- the reference has no backend function for these: repdl/optim.py:56-83
  * writes Adam as a sequence of PyTorch tensor operations around ops.sqrt and a true

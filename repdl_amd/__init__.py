@@ -32,20 +32,25 @@ def _bn_args(m):
     return (m.num_features, m.eps, m.momentum, m.weight is not None, m.track_running_stats)
 
 
-def from_torch_module(m: torch.nn.Module) -> torch.nn.Module:
+def from_torch_module(m: torch.nn.Module, language_layers: bool = False) -> torch.nn.Module:
     """Return a copy of ``m`` in which every ``torch.nn`` layer that has a
     reproducible counterpart is replaced by it, weights included.
 
     Same rules as RepDL's ``repdl/__init__.py:15-65``: the match is on the exact
     type (subclasses are left alone); ``Sequential`` is rebuilt; any other module
-    is shallow-copied and its children converted recursively."""
+    is shallow-copied and its children converted recursively.
+
+    ``language_layers``: also replace LayerNorm and Dropout, which the reference leaves as they
+    are.  Each new Dropout draws its seed from PyTorch's CPU generator, in the order of the modules."""
     if not isinstance(m, torch.nn.Module):
         raise TypeError("from_torch_module expects a torch.nn.Module")
     kind = type(m)
     if kind is torch.nn.Sequential:
-        return torch.nn.Sequential(*[from_torch_module(child) for child in m])
+        return torch.nn.Sequential(*[from_torch_module(child, language_layers) for child in m])
     if kind is torch.nn.CrossEntropyLoss:
         return nn.CrossEntropyLoss(m.weight, None, m.ignore_index, None, m.reduction, m.label_smoothing)
+    if language_layers and kind is torch.nn.Dropout:
+        return nn.Dropout(m.p).train(m.training)
     if kind is torch.nn.Linear:
         new = nn.Linear(m.in_features, m.out_features, m.bias is not None)
     elif kind is torch.nn.Conv2d:
@@ -55,10 +60,13 @@ def from_torch_module(m: torch.nn.Module) -> torch.nn.Module:
         new = nn.BatchNorm1d(*_bn_args(m))
     elif kind is torch.nn.BatchNorm2d:
         new = nn.BatchNorm2d(*_bn_args(m))
+    elif language_layers and kind is torch.nn.LayerNorm:
+        new = nn.LayerNorm(m.normalized_shape, m.eps, m.elementwise_affine, m.bias is not None,
+                           dtype=None if m.weight is None else m.weight.dtype)
     else:
         new = copy(m)
         for name, child in m.named_children():
-            setattr(new, name, from_torch_module(child))
+            setattr(new, name, from_torch_module(child, language_layers))
         return new
     new.load_state_dict(m.state_dict())
     return new

@@ -16,6 +16,8 @@ _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _INT = ctypes.c_int
 _F32 = ctypes.c_float
+_F64 = ctypes.c_double
+_U64 = ctypes.c_uint64
 
 
 
@@ -62,6 +64,14 @@ SIGNATURES = {
     "repdl_hip_bn_apply": [_P] * 6 + [_I64] * 3 + [_P],
     "repdl_hip_bn_gvar_term": [_P] * 5 + [_I64] * 3 + [_P],
     "repdl_hip_bn_gweight_term": [_P] * 5 + [_I64] * 3 + [_P],
+    "repdl_hip_layer_norm": [_P] * 6 + [_I64, _I64, _F32, _INT, _INT, _P],
+    "repdl_hip_layer_norm_grad": [_P] * 8 + [_I64, _I64, _INT, _INT, _P],
+    "repdl_hip_layer_norm_grad_ws": [_P] * 8 + [_I64, _I64, _INT, _INT, _P, ctypes.c_size_t, _P],
+    "repdl_hip_dropout": [_P, _P, _P, _I64, _F64, _P, _U64, _U64, _INT, _P],
+    "repdl_hip_dropout_next_call": [_P, _P, _P],
+    "repdl_hip_preference_loss": [_P] * 7 + [_I64] * 5 + [_F64, _F64, _I64, _INT, _P],
+    "repdl_hip_preference_loss_ws": [_P] * 7 + [_I64] * 5 + [_F64, _F64, _I64, _INT, _P, ctypes.c_size_t, _P],
+    "repdl_hip_preference_loss_grad": [_P] * 6 + [_I64] * 6 + [_INT, _P],
     "repdl_hip_adam_step": [ctypes.POINTER(AdamTensor), _INT] + [_F32] * 6 + [_P],
     "repdl_hip_sgd_step": [ctypes.POINTER(SgdTensor), _INT, _F32, _P],
     "repdl_hip_mfma_selftest": [_I64, _I64, ctypes.c_uint64, ctypes.POINTER(ctypes.c_uint64)],
@@ -78,6 +88,8 @@ SIZE_QUERIES = {
     "repdl_hip_sum2d_dim1_workspace_bytes": [_I64, _I64],
     "repdl_hip_sum4d_dim023_workspace_bytes": [_I64] * 4,
     "repdl_hip_cross_entropy_workspace_bytes": [_I64, _I64],
+    "repdl_hip_layer_norm_grad_workspace_bytes": [_I64, _I64],
+    "repdl_hip_preference_loss_workspace_bytes": [_I64] * 3,
     "repdl_hip_scratch_bytes": [],
 }
 

@@ -3,7 +3,8 @@
 the same ten functions with the same positional signatures, tensors in and a new
 tensor out, plus the elementwise operators (``exp``, ``log``, ``sqrt``, ``div``,
 ``div_scalar``), ``mm_bias`` / ``conv2d_bias`` (the layer's bias added in the
-kernel's epilogue) and the fused elementwise passes of batch normalisation.  ``repdl_amd.backend.hip`` serves these when the compiled binding
+kernel's epilogue), the fused elementwise passes of batch normalisation, and layer
+normalisation, dropout and the preference loss.  ``repdl_amd.backend.hip`` serves these when the compiled binding
 (csrc/bind.cpp) has not been built; both call the same library.
 
 Each function validates its tensors (float32, on the GPU, made contiguous),
@@ -306,4 +307,174 @@ def bn_gweight_term(input, mean, std, grad_output) -> torch.Tensor:
     with torch.cuda.device(x.device):
         _lib.call("repdl_hip_bn_gweight_term", _ptr(x), _ptr(m), _ptr(s), _ptr(g), _ptr(out), outer, channels, inner,
                   _stream(x))
+    return out
+
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _check_any(t: torch.Tensor, name: str) -> torch.Tensor:
+    """A tensor of one of the types that layer norm, dropout and the preference loss take."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s must be a torch.Tensor" % name)
+    if not t.is_cuda:
+        raise RuntimeError("%s must be on the GPU (this backend has no CPU path)" % name)
+    if t.dtype not in _DTYPES:
+        raise RuntimeError("%s must be float32, bfloat16 or float16, got %s" % (name, t.dtype))
+    return t.contiguous()
+
+
+def _opt(t):
+    return None if t is None else _ptr(t)
+
+
+def _norm_param(p, name: str, x: torch.Tensor, n: int, code):
+    """weight or bias of a layer norm: [n] of the input's type or float32 on the same device, or None -> tensor, type code"""
+    if p is None:
+        return None, code
+    t = _check_any(p, name)
+    _same_device(t, x)
+    if t.numel() != n:
+        raise RuntimeError("%s has %d elements for rows of %d" % (name, t.numel(), n))
+    if t.dtype not in (torch.float32, x.dtype):
+        raise RuntimeError("%s must be %s like the input, or float32" % (name, x.dtype))
+    if code is not None and code != _DTYPES[t.dtype]:
+        raise RuntimeError("weight and bias differ in type")
+    return t, _DTYPES[t.dtype]
+
+
+def _norm_rows(x: torch.Tensor, n: int) -> int:
+    if n < 0 or (x.numel() != 0 if n == 0 else x.numel() % n != 0):
+        raise RuntimeError("layer_norm: %d elements are no whole rows of %d" % (x.numel(), n))
+    return 0 if n == 0 else x.numel() // n
+
+
+def layer_norm(input, n: int, weight, bias, eps: float, stats: bool):
+    """Rows of n elements normalised -> output and, with ``stats``, mean and rstd of every row (else None)."""
+    x = _check_any(input, "input")
+    rows = _norm_rows(x, n)
+    w, code = _norm_param(weight, "weight", x, n, None)
+    b, code = _norm_param(bias, "bias", x, n, code)
+    out = torch.empty_like(x)
+    mean, rstd = (torch.empty((rows,), dtype=torch.float32, device=x.device) if stats else None for _ in range(2))
+    with torch.cuda.device(x.device):
+        _lib.call("repdl_hip_layer_norm", _ptr(x), _opt(w), _opt(b), _ptr(out), _opt(mean), _opt(rstd), rows, n, eps, _DTYPES[x.dtype],
+                  code or 0, _stream(x))
+    return out, mean, rstd
+
+
+def layer_norm_grad(grad_output, input, mean, rstd, n: int, weight, param_like, need_input: bool, need_weight: bool, need_bias: bool):
+    """The gradients of layer_norm that are asked for (else None); those of weight and bias are [n], of param_like's type."""
+    x, gy = _check_any(input, "input"), _check_any(grad_output, "grad_output")
+    if gy.shape != x.shape or gy.dtype != x.dtype:
+        raise RuntimeError("grad_output and input differ in shape or type")
+    _same_device(gy, x)
+    rows = _norm_rows(x, n)
+    m, r = _check(mean, "mean", 1), _check(rstd, "rstd", 1)
+    if m.shape[0] != rows or r.shape[0] != rows:
+        raise RuntimeError("mean and rstd are not those of the input's %d rows" % rows)
+    _same_device(m, x)
+    _same_device(r, x)
+    w, code = _norm_param(weight, "weight", x, n, None)
+    _, code = _norm_param(param_like, "param_like", x, n, code)
+    kind = x.dtype if code else torch.float32
+    gx = torch.empty_like(x) if need_input else None
+    gw = torch.empty((n,), dtype=kind, device=x.device) if need_weight else None
+    gb = torch.empty((n,), dtype=kind, device=x.device) if need_bias else None
+    with torch.cuda.device(x.device):
+        work, wp, wn = None, None, ctypes.c_size_t(0)
+        if need_weight or need_bias:
+            work, wp, wn = _scratch("repdl_hip_layer_norm_grad_workspace_bytes", x, rows, n)
+        _lib.call("repdl_hip_layer_norm_grad_ws", _ptr(gy), _ptr(x), _opt(w), _ptr(m), _ptr(r), _opt(gx), _opt(gw), _opt(gb), rows, n,
+                  _DTYPES[x.dtype], code or 0, wp, wn, _stream(x))
+    return gx, gw, gb
+
+
+def _dropout_state(state: torch.Tensor) -> _P:
+    if not (state.is_cuda and state.dtype == torch.int64 and tuple(state.shape) == (2,) and state.is_contiguous()):
+        raise RuntimeError("the state of dropout is an int64 tensor (seed, call) on the GPU")
+    return _ptr(state)
+
+
+def dropout(input, residual, p: float, state, seed: int, call: int) -> torch.Tensor:
+    """Dropout (added to residual, if there is one) for the call (seed, call), read from ``state`` on the device where there is one."""
+    x = _check_any(input, "input")
+    if not 0.0 <= p <= 1.0:
+        raise RuntimeError("dropout probability has to be between 0 and 1, but got %s" % p)
+    r = None
+    if residual is not None:
+        r = _check_any(residual, "residual")
+        _same_device(r, x)
+        if r.shape != x.shape or r.dtype != x.dtype:
+            raise RuntimeError("residual and input differ in shape or type")
+    if state is not None:
+        _same_device(state, x)
+    out = torch.empty_like(x)
+    with torch.cuda.device(x.device):
+        _lib.call("repdl_hip_dropout", _ptr(x), _opt(r), _ptr(out), x.numel(), p, None if state is None else _dropout_state(state), seed, call,
+                  _DTYPES[x.dtype], _stream(x))
+    return out
+
+
+def dropout_next_call(state: torch.Tensor) -> torch.Tensor:
+    """A copy of ``state``, whose call number is then one more."""
+    sp = _dropout_state(state)
+    used = torch.empty_like(state)
+    with torch.cuda.device(state.device):
+        _lib.call("repdl_hip_dropout_next_call", sp, _ptr(used), _stream(state))
+    return used
+
+
+def _pref_logits(logits: torch.Tensor, target: torch.Tensor) -> torch.Tensor:
+    """Logits of a preference loss: rows of contiguous elements, any strides between sequences and steps."""
+    if not logits.is_cuda:
+        raise RuntimeError("logits must be on the GPU (this backend has no CPU path)")
+    if logits.dtype not in _DTYPES:
+        raise RuntimeError("logits must be float32, bfloat16 or float16, got %s" % logits.dtype)
+    if logits.dim() != 3:
+        raise RuntimeError("logits must have 3 dimensions (sequence, step, vocabulary), got %d" % logits.dim())
+    if logits.shape[0] < 2 or logits.shape[0] % 2:
+        raise RuntimeError("logits: the preferred answers, then as many others (got %d sequences)" % logits.shape[0])
+    if logits.shape[2] < 1:
+        raise RuntimeError("logits: an empty vocabulary")
+    if not target.is_cuda or target.dtype != torch.int64:
+        raise RuntimeError("target must be int64 on the GPU")
+    if tuple(target.shape) != tuple(logits.shape[:2]):
+        raise RuntimeError("target must be %s like the logits' rows" % (list(logits.shape[:2]),))
+    _same_device(target, logits)
+    return logits if logits.stride(2) == 1 or logits.shape[2] == 1 else logits.contiguous()
+
+
+def preference_loss(logits, target, ref_logps, beta: float, label_smoothing: float, ignore_index: int, grad: bool):
+    """Loss, log probabilities of the sequences, and (with ``grad``) row statistics and coefficients for the backward pass."""
+    x, t = _pref_logits(logits, target), target.contiguous()
+    seqs, steps, vocab = x.shape
+    ref = None
+    if ref_logps is not None:
+        ref = _check(ref_logps, "ref_logps", 1)
+        _same_device(ref, x)
+        if ref.shape[0] != seqs:
+            raise RuntimeError("ref_logps has %d elements for %d sequences" % (ref.shape[0], seqs))
+    loss, logps = torch.empty((), dtype=torch.float32, device=x.device), torch.empty((seqs,), dtype=torch.float32, device=x.device)
+    stats = torch.empty((seqs, steps, 2), dtype=torch.float32, device=x.device) if grad else None
+    coef = torch.empty((seqs,), dtype=torch.float32, device=x.device) if grad else None
+    with torch.cuda.device(x.device):
+        work, wp, wn = _scratch("repdl_hip_preference_loss_workspace_bytes", x, seqs // 2, steps, vocab)
+        _lib.call("repdl_hip_preference_loss_ws", _ptr(x), _ptr(t), _opt(ref), _ptr(loss), _ptr(logps), _opt(stats), _opt(coef), seqs // 2,
+                  steps, vocab, x.stride(0), x.stride(1), beta, label_smoothing, ignore_index, _DTYPES[x.dtype], wp, wn, _stream(x))
+    return loss, logps, stats, coef
+
+
+def preference_loss_grad(logits, target, row_stats, coef, grad_loss, ignore_index: int) -> torch.Tensor:
+    x, t = _pref_logits(logits, target), target.contiguous()
+    seqs, steps, vocab = x.shape
+    st, c, g = _check(row_stats, "row_stats", 3), _check(coef, "coef", 1), _check(grad_loss, "grad_loss", 0)
+    if tuple(st.shape) != (seqs, steps, 2) or c.shape[0] != seqs:
+        raise RuntimeError("row_stats and coef are not those of these logits")
+    for v in (st, c, g):
+        _same_device(v, x)
+    out = torch.empty((seqs, steps, vocab), dtype=x.dtype, device=x.device)
+    with torch.cuda.device(x.device):
+        _lib.call("repdl_hip_preference_loss_grad", _ptr(x), _ptr(t), _ptr(st), _ptr(c), _ptr(g), _ptr(out), seqs // 2, steps, vocab,
+                  x.stride(0), x.stride(1), ignore_index, _DTYPES[x.dtype], _stream(x))
     return out

@@ -4,7 +4,8 @@
 // convolution.cu:153-155, 259-262, 359-362, 385-387; summation.cu:149-155;
 // softmax.cpp:15, 28; cross_entropy.cpp:15, 31), plus exp / log / sqrt / div / div_scalar and
 // mm_bias / conv2d_bias (the layer's bias added in the kernel's epilogue) and the fused elementwise
-// passes of batch normalisation (bn_apply, bn_gvar_term, bn_gweight_term).
+// passes of batch normalisation (bn_apply, bn_gvar_term, bn_gweight_term), layer normalisation, dropout and
+// the preference loss with their gradients.
 // It is the only file of this library that knows about PyTorch: every function checks its
 // tensors, allocates the output on the input's device, and hands raw pointers and the current
 // stream to the C ABI of include/repdl_hip.h.  Host C++ only; built with the host compiler
@@ -354,6 +355,220 @@ torch::Tensor bn_gweight_term(const torch::Tensor &input, const torch::Tensor &m
     return out;
 }
 
+namespace
+{
+// the element types of the operators below, by their code in the C ABI
+int dtype_code(const torch::Tensor &t, const char *name)
+{
+    const auto k = t.scalar_type();
+    TORCH_CHECK(k == torch::kFloat || k == torch::kBFloat16 || k == torch::kHalf, name, " must be float32, bfloat16 or float16, got ", k);
+    return k == torch::kFloat ? REPDL_F32 : k == torch::kBFloat16 ? REPDL_BF16 : REPDL_F16;
+}
+
+torch::Tensor checked_any(const torch::Tensor &t, const char *name)
+{
+    TORCH_CHECK(t.is_cuda(), name, " must be on the GPU (this backend has no CPU path)");
+    dtype_code(t, name);
+    return t.contiguous();
+}
+
+// weight or bias of a layer norm: [n] of the input's type or float32 on the same device, or none
+const void *norm_param(const c10::optional<torch::Tensor> &p, torch::Tensor &hold, const char *name, const torch::Tensor &x, int64_t n,
+                       int &code)
+{
+    if (!p.has_value())
+        return nullptr;
+    hold = checked_any(*p, name);
+    same_device(hold, x);
+    TORCH_CHECK(hold.numel() == n, name, " has ", hold.numel(), " elements for rows of ", n);
+    const int c = dtype_code(hold, name);
+    TORCH_CHECK(c == REPDL_F32 || hold.scalar_type() == x.scalar_type(), name, " must be ", x.scalar_type(), " like the input, or float32");
+    TORCH_CHECK(code < 0 || code == c, "weight and bias differ in type");
+    code = c;
+    return hold.data_ptr();
+}
+
+int64_t norm_rows(const torch::Tensor &x, int64_t n)
+{
+    TORCH_CHECK(n >= 0 && (n == 0 ? x.numel() == 0 : x.numel() % n == 0), "layer_norm: ", x.numel(), " elements are no whole rows of ", n);
+    return n == 0 ? 0 : x.numel() / n;
+}
+} // namespace
+
+// rows of n elements normalised; with `stats` also mean and rstd of every row (else undefined)
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> layer_norm(const torch::Tensor &input, int64_t n,
+                                                                   const c10::optional<torch::Tensor> &weight,
+                                                                   const c10::optional<torch::Tensor> &bias, double eps, bool stats)
+{
+    const auto x = checked_any(input, "input");
+    const int64_t rows = norm_rows(x, n);
+    const DeviceGuard guard(x.device());
+    torch::Tensor hw, hb, mean, rstd;
+    int code = -1;
+    const void *w = norm_param(weight, hw, "weight", x, n, code), *b = norm_param(bias, hb, "bias", x, n, code);
+    auto out = torch::empty_like(x);
+    if (stats)
+    {
+        mean = torch::empty({rows}, x.options().dtype(torch::kFloat));
+        rstd = torch::empty({rows}, x.options().dtype(torch::kFloat));
+    }
+    ok(repdl_hip_layer_norm(x.data_ptr(), w, b, out.data_ptr(), stats ? mean.data_ptr<float>() : nullptr,
+                            stats ? rstd.data_ptr<float>() : nullptr, rows, n, (float)eps, dtype_code(x, "input"),
+                            code < 0 ? REPDL_F32 : code, current_stream()),
+       "repdl_hip_layer_norm");
+    return {out, mean, rstd};
+}
+
+// the gradients of layer_norm that are asked for (the others are undefined); those of weight and bias are [n], of param_like's type
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> layer_norm_grad(const torch::Tensor &grad_output, const torch::Tensor &input,
+                                                                        const torch::Tensor &mean, const torch::Tensor &rstd, int64_t n,
+                                                                        const c10::optional<torch::Tensor> &weight,
+                                                                        const c10::optional<torch::Tensor> &param_like, bool need_input,
+                                                                        bool need_weight, bool need_bias)
+{
+    const auto x = checked_any(input, "input"), gy = checked_any(grad_output, "grad_output");
+    TORCH_CHECK(gy.sizes() == x.sizes() && gy.scalar_type() == x.scalar_type(), "grad_output and input differ in shape or type");
+    same_device(gy, x);
+    const int64_t rows = norm_rows(x, n);
+    const auto m = checked(mean, "mean", 1), r = checked(rstd, "rstd", 1);
+    TORCH_CHECK(m.size(0) == rows && r.size(0) == rows, "mean and rstd are not those of the input's ", rows, " rows");
+    same_device(m, x);
+    same_device(r, x);
+    const DeviceGuard guard(x.device());
+    torch::Tensor hw, hp, gx, gw, gb;
+    int code = -1;
+    const void *w = norm_param(weight, hw, "weight", x, n, code);
+    norm_param(param_like, hp, "param_like", x, n, code);
+    const auto kind = code < 0 ? torch::kFloat : code == REPDL_F32 ? torch::kFloat : x.scalar_type();
+    if (need_input)
+        gx = torch::empty_like(x);
+    if (need_weight)
+        gw = torch::empty({n}, x.options().dtype(kind));
+    if (need_bias)
+        gb = torch::empty({n}, x.options().dtype(kind));
+    const Scratch work(need_weight || need_bias ? repdl_hip_layer_norm_grad_workspace_bytes(rows, n) : 0, x);
+    ok(repdl_hip_layer_norm_grad_ws(gy.data_ptr(), x.data_ptr(), w, m.data_ptr<float>(), r.data_ptr<float>(),
+                                    need_input ? gx.data_ptr() : nullptr, need_weight ? gw.data_ptr() : nullptr,
+                                    need_bias ? gb.data_ptr() : nullptr, rows, n, dtype_code(x, "input"), code < 0 ? REPDL_F32 : code,
+                                    work.ptr(), work.bytes, current_stream()),
+       "repdl_hip_layer_norm_grad_ws");
+    return {gx, gw, gb};
+}
+
+namespace
+{
+const int64_t *dropout_state(const torch::Tensor &state)
+{
+    TORCH_CHECK(state.is_cuda() && state.scalar_type() == torch::kLong && state.dim() == 1 && state.size(0) == 2 && state.is_contiguous(),
+                "the state of dropout is an int64 tensor (seed, call) on the GPU");
+    return state.data_ptr<int64_t>();
+}
+} // namespace
+
+// dropout (added to residual, if there is one) for the call (seed, call), read from `state` on the device where there is one
+torch::Tensor dropout(const torch::Tensor &input, const c10::optional<torch::Tensor> &residual, double p,
+                      const c10::optional<torch::Tensor> &state, uint64_t seed, uint64_t call)
+{
+    const auto x = checked_any(input, "input");
+    TORCH_CHECK(p >= 0.0 && p <= 1.0, "dropout probability has to be between 0 and 1, but got ", p);
+    torch::Tensor r;
+    if (residual.has_value())
+    {
+        r = checked_any(*residual, "residual");
+        same_device(r, x);
+        TORCH_CHECK(r.sizes() == x.sizes() && r.scalar_type() == x.scalar_type(), "residual and input differ in shape or type");
+    }
+    if (state.has_value())
+        same_device(*state, x);
+    const DeviceGuard guard(x.device());
+    auto out = torch::empty_like(x);
+    ok(repdl_hip_dropout(x.data_ptr(), r.defined() ? r.data_ptr() : nullptr, out.data_ptr(), x.numel(), p,
+                         state.has_value() ? dropout_state(*state) : nullptr, seed, call, dtype_code(x, "input"), current_stream()),
+       "repdl_hip_dropout");
+    return out;
+}
+
+// a copy of `state`, whose call number is then one more
+torch::Tensor dropout_next_call(const torch::Tensor &state)
+{
+    dropout_state(state);
+    const DeviceGuard guard(state.device());
+    auto used = torch::empty_like(state);
+    ok(repdl_hip_dropout_next_call(state.data_ptr<int64_t>(), used.data_ptr<int64_t>(), current_stream()), "repdl_hip_dropout_next_call");
+    return used;
+}
+
+namespace
+{
+// logits of a preference loss: rows of contiguous elements, any strides between sequences and steps
+torch::Tensor pref_logits(const torch::Tensor &logits, const torch::Tensor &target)
+{
+    TORCH_CHECK(logits.is_cuda(), "logits must be on the GPU (this backend has no CPU path)");
+    dtype_code(logits, "logits");
+    TORCH_CHECK(logits.dim() == 3, "logits must have 3 dimensions (sequence, step, vocabulary), got ", logits.dim());
+    TORCH_CHECK(logits.size(0) >= 2 && logits.size(0) % 2 == 0, "logits: the preferred answers, then as many others (got ", logits.size(0),
+                " sequences)");
+    TORCH_CHECK(logits.size(2) >= 1, "logits: an empty vocabulary");
+    TORCH_CHECK(target.is_cuda() && target.scalar_type() == torch::kLong, "target must be int64 on the GPU");
+    TORCH_CHECK(target.dim() == 2 && target.size(0) == logits.size(0) && target.size(1) == logits.size(1), "target must be [", logits.size(0),
+                ", ", logits.size(1), "] like the logits' rows");
+    same_device(target, logits);
+    return logits.stride(2) == 1 || logits.size(2) == 1 ? logits : logits.contiguous();
+}
+} // namespace
+
+// loss, log probabilities of the sequences, and (with `grad`) row statistics and coefficients for the backward pass
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> preference_loss(const torch::Tensor &logits, const torch::Tensor &target,
+                                                                                       const c10::optional<torch::Tensor> &ref_logps,
+                                                                                       double beta, double label_smoothing,
+                                                                                       int64_t ignore_index, bool grad)
+{
+    const auto x = pref_logits(logits, target), t = target.contiguous();
+    const int64_t seqs = x.size(0), steps = x.size(1), vocab = x.size(2);
+    torch::Tensor ref, stats, coef;
+    if (ref_logps.has_value())
+    {
+        ref = checked(*ref_logps, "ref_logps", 1);
+        same_device(ref, x);
+        TORCH_CHECK(ref.size(0) == seqs, "ref_logps has ", ref.size(0), " elements for ", seqs, " sequences");
+    }
+    const DeviceGuard guard(x.device());
+    const auto f32 = x.options().dtype(torch::kFloat);
+    auto loss = torch::empty({}, f32), logps = torch::empty({seqs}, f32);
+    if (grad)
+    {
+        stats = torch::empty({seqs, steps, 2}, f32);
+        coef = torch::empty({seqs}, f32);
+    }
+    const Scratch work(repdl_hip_preference_loss_workspace_bytes(seqs / 2, steps, vocab), x);
+    ok(repdl_hip_preference_loss_ws(x.data_ptr(), t.data_ptr<int64_t>(), ref.defined() ? ref.data_ptr<float>() : nullptr,
+                                    loss.data_ptr<float>(), logps.data_ptr<float>(), grad ? stats.data_ptr<float>() : nullptr,
+                                    grad ? coef.data_ptr<float>() : nullptr, seqs / 2, steps, vocab, x.stride(0), x.stride(1), beta,
+                                    label_smoothing, ignore_index, dtype_code(x, "logits"), work.ptr(), work.bytes, current_stream()),
+       "repdl_hip_preference_loss_ws");
+    return {loss, logps, stats, coef};
+}
+
+torch::Tensor preference_loss_grad(const torch::Tensor &logits, const torch::Tensor &target, const torch::Tensor &row_stats,
+                                   const torch::Tensor &coef, const torch::Tensor &grad_loss, int64_t ignore_index)
+{
+    const auto x = pref_logits(logits, target), t = target.contiguous();
+    const int64_t seqs = x.size(0), steps = x.size(1), vocab = x.size(2);
+    const auto st = checked(row_stats, "row_stats", 3), c = checked(coef, "coef", 1), g = checked(grad_loss, "grad_loss", 0);
+    TORCH_CHECK(st.size(0) == seqs && st.size(1) == steps && st.size(2) == 2 && c.size(0) == seqs,
+                "row_stats and coef are not those of these logits");
+    same_device(st, x);
+    same_device(c, x);
+    same_device(g, x);
+    const DeviceGuard guard(x.device());
+    auto out = torch::empty({seqs, steps, vocab}, x.options());
+    ok(repdl_hip_preference_loss_grad(x.data_ptr(), t.data_ptr<int64_t>(), st.data_ptr<float>(), c.data_ptr<float>(), g.data_ptr<float>(),
+                                      out.data_ptr(), seqs / 2, steps, vocab, x.stride(0), x.stride(1), ignore_index,
+                                      dtype_code(x, "logits"), current_stream()),
+       "repdl_hip_preference_loss_grad");
+    return out;
+}
+
 } // namespace hip
 } // namespace repdl
 
@@ -387,4 +602,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("bn_apply", &h::bn_apply);
     m.def("bn_gvar_term", &h::bn_gvar_term);
     m.def("bn_gweight_term", &h::bn_gweight_term);
+    m.def("layer_norm", &h::layer_norm);
+    m.def("layer_norm_grad", &h::layer_norm_grad);
+    m.def("dropout", &h::dropout);
+    m.def("dropout_next_call", &h::dropout_next_call);
+    m.def("preference_loss", &h::preference_loss);
+    m.def("preference_loss_grad", &h::preference_loss_grad);
 }

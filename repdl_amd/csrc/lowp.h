@@ -1,0 +1,100 @@
+// Tensors of binary32, bfloat16 or binary16 elements that are computed on in binary32: loads widen exactly, stores
+// round once (to nearest even).  Shared by the kernels of layer normalisation, dropout and the preference loss.
+#pragma once
+
+#include "common.h"
+
+// Widening and rounding of one element, by the type's code in the C ABI.
+template <int DT>
+struct LowpType;
+
+template <>
+struct LowpType<REPDL_F32>
+{
+    typedef float T;
+    __device__ static __forceinline__ float widen(float v) { return v; }
+    __device__ static __forceinline__ float narrow(float v) { return v; }
+};
+
+template <>
+struct LowpType<REPDL_BF16>
+{
+    typedef __bf16 T;
+    __device__ static __forceinline__ float widen(__bf16 v) { return (float)v; }
+    __device__ static __forceinline__ __bf16 narrow(float v) { return (__bf16)v; }
+};
+
+template <>
+struct LowpType<REPDL_F16>
+{
+    typedef _Float16 T;
+    __device__ static __forceinline__ float widen(_Float16 v) { return (float)v; }
+    __device__ static __forceinline__ _Float16 narrow(float v) { return (_Float16)v; }
+};
+
+// 16 bytes of a tensor, the unit that a lane moves: `G` elements.
+template <int DT>
+struct Lowp
+{
+    typedef typename LowpType<DT>::T T;
+    static constexpr int G = 16 / (int)sizeof(T);
+    typedef uint32_t Raw __attribute__((ext_vector_type(4)));
+
+    // Rows may start at any element (an odd row length in a 16-bit type): the hardware takes a 16-byte access on any
+    // boundary, so there is one path for aligned and unaligned rows, and the order of a sum never depends on an address.
+    __device__ static __forceinline__ Raw load_raw(const T *p)
+    {
+        Raw r;
+        __builtin_memcpy(&r, p, 16);
+        return r;
+    }
+    __device__ static __forceinline__ void unpack(const Raw &r, float *v)
+    {
+        T t[G];
+        __builtin_memcpy(t, &r, 16);
+#pragma unroll
+        for (int k = 0; k < G; k++)
+            v[k] = LowpType<DT>::widen(t[k]);
+    }
+    __device__ static __forceinline__ Raw pack(const float *v)
+    {
+        T t[G];
+#pragma unroll
+        for (int k = 0; k < G; k++)
+            t[k] = LowpType<DT>::narrow(v[k]);
+        Raw r;
+        __builtin_memcpy(&r, t, 16);
+        return r;
+    }
+
+    // elements c .. c+G-1 of a row of n; those past the end come as `fill`
+    __device__ static __forceinline__ void load(const T *row, int64_t c, int64_t n, float fill, float *v)
+    {
+        if (c + G <= n)
+            unpack(load_raw(row + c), v);
+        else
+        {
+#pragma unroll
+            for (int k = 0; k < G; k++)
+                v[k] = c + k < n ? LowpType<DT>::widen(row[c + k]) : fill;
+        }
+    }
+    __device__ static __forceinline__ void store(T *row, int64_t c, int64_t n, const float *v)
+    {
+        if (c + G <= n)
+        {
+            const Raw r = pack(v);
+            __builtin_memcpy(row + c, &r, 16);
+        }
+        else
+        {
+#pragma unroll
+            for (int k = 0; k < G; k++)
+                if (c + k < n)
+                    row[c + k] = LowpType<DT>::narrow(v[k]);
+        }
+    }
+};
+
+static inline bool repdl_known_dtype(int dtype) { return dtype == REPDL_F32 || dtype == REPDL_BF16 || dtype == REPDL_F16; }
+static inline int64_t repdl_dtype_bytes(int dtype) { return dtype == REPDL_F32 ? 4 : 2; }

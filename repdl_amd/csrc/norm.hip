@@ -1,0 +1,678 @@
+// Layer normalisation, forward and backward.
+//
+//   mean = (1/N) sum_j x_j,  var = (1/N) sum_j (x_j - mean)^2,  rstd = 1 / sqrt(var + eps)
+//   xh_j = (x_j - mean) rstd,  y_j = xh_j w_j + b_j
+//   g_j = gy_j w_j,  gx_j = rstd ((g_j - mean(g)) - xh_j mean(g xh))
+//   gw_j = sum_i gy_ij xh_ij,  gb_j = sum_i gy_ij
+//
+// Every operation above is one IEEE binary32 operation (nothing is fused; the square root and the reciprocal are the
+// correctly rounded ones of crmath.h; "(1/N)" is one multiplication by float(1/N), as in the library's averages), so a
+// result is a function of the inputs and of the order of the sums alone.  That order is fixed by the row length, the type
+// and -- for gw and gb -- the number of rows; the device, the stream, the addresses and the other rows have no part in it.
+//
+// The two passes over a row (mean, then centred squares) read it from registers: one thread holds E = 16 or 32 of its
+// elements, as 16-byte granules TPR granules apart, TPR threads a row.  Bound: HBM.
+#include "lowp.h"
+#include "crmath.h"
+
+namespace
+{
+// Threads per row: the smallest power of two, at least 4, that holds the row in E elements per thread.
+__host__ __device__ constexpr int ln_threads_per_row(int64_t N, int E)
+{
+    int t = 4;
+    while ((int64_t)t * E < N)
+        t *= 2;
+    return t;
+}
+constexpr int LN_E = 16;
+constexpr int LN_MAX_TPR = 1024; // rows of more than LN_MAX_TPR * LN_E elements are read from memory for every pass
+constexpr int64_t LN_MAX_ONCHIP = (int64_t)LN_MAX_TPR * LN_E;
+
+// Sum over the TPR threads of a row of K values each, in every thread of the row: a butterfly inside the wave, then the
+// waves' sums in order.  `scratch`: K * (TPR / 64) floats of LDS per row team, free again at the next call's second barrier;
+// callers alternate between two halves.
+template <int TPR, int K>
+__device__ __forceinline__ void team_sum(float (&v)[K], float *scratch, int j)
+{
+    constexpr int W = TPR < 64 ? TPR : 64;
+#pragma unroll
+    for (int off = 1; off < W; off <<= 1)
+    {
+#pragma unroll
+        for (int k = 0; k < K; k++)
+            v[k] = v[k] + __shfl_xor(v[k], off, 64);
+    }
+    if (TPR > 64)
+    {
+        constexpr int NW = TPR / 64;
+        if ((j & 63) == 0)
+        {
+#pragma unroll
+            for (int k = 0; k < K; k++)
+                scratch[k * NW + (j >> 6)] = v[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < K; k++)
+        {
+            float s = scratch[k * NW];
+#pragma unroll
+            for (int w = 1; w < NW; w++)
+                s = s + scratch[k * NW + w];
+            v[k] = s;
+        }
+    }
+}
+
+// Sum of a granule's elements: pairs, pairs of pairs.
+template <int G>
+__device__ __forceinline__ float granule_sum(const float *v)
+{
+    float t[G];
+#pragma unroll
+    for (int k = 0; k < G; k++)
+        t[k] = v[k];
+#pragma unroll
+    for (int step = 1; step < G; step <<= 1)
+    {
+#pragma unroll
+        for (int k = 0; k + step < G; k += 2 * step)
+            t[k] = t[k] + t[k + step];
+    }
+    return t[0];
+}
+
+__device__ __forceinline__ float ln_rstd(float var, float eps) { return crm_div(1.0f, crm_sqrt(var + eps)); }
+
+// Parameters are read in granules of the activation's element count, whatever their own type.
+template <int G, int PDT>
+__device__ __forceinline__ void load_param(const typename LowpType<PDT>::T *p, int64_t c, int64_t n, float fill, float *v)
+{
+    typedef Lowp<PDT> P;
+    if (p == nullptr)
+    {
+#pragma unroll
+        for (int k = 0; k < G; k++)
+            v[k] = fill;
+        return;
+    }
+    if (P::G == G)
+        P::load(p, c, n, 0.0f, v);
+    else // binary32 parameters of a 16-bit activation: two granules
+    {
+        P::load(p, c, n, 0.0f, v);
+        P::load(p, c + P::G, n, 0.0f, v + G - P::G);
+    }
+}
+
+template <int DT, int PDT, int TPR, int E>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_kernel(
+    const typename LowpType<DT>::T *__restrict__ x, const typename LowpType<PDT>::T *__restrict__ w,
+    const typename LowpType<PDT>::T *__restrict__ b, typename LowpType<DT>::T *__restrict__ y, float *__restrict__ mean_out,
+    float *__restrict__ rstd_out, int64_t M, int N, float inv_n, float eps)
+{
+    typedef Lowp<DT> L;
+    constexpr int G = L::G, GPT = E / G;
+    constexpr int THREADS = TPR < 256 ? 256 : TPR, TEAMS = THREADS / TPR;
+    __shared__ float scratch[2][TEAMS][TPR / 64 + 1];
+    const int tid = threadIdx.x, team = tid / TPR, j = tid % TPR;
+    const int64_t row = (int64_t)blockIdx.x * TEAMS + team;
+    const bool live = row < M;
+    const typename L::T *xr = x + (live ? row : M - 1) * N;
+
+    float v[GPT][G];
+#pragma unroll
+    for (int i = 0; i < GPT; i++)
+        L::load(xr, (int64_t)(i * TPR + j) * G, N, 0.0f, v[i]);
+    float s[1] = {0.0f};
+#pragma unroll
+    for (int i = 0; i < GPT; i++)
+        s[0] = s[0] + granule_sum<G>(v[i]);
+    team_sum<TPR, 1>(s, scratch[0][team], j);
+    const float mean = s[0] * inv_n;
+    float q[1] = {0.0f};
+#pragma unroll
+    for (int i = 0; i < GPT; i++)
+    {
+        const int c = (i * TPR + j) * G;
+        float sq[G];
+#pragma unroll
+        for (int k = 0; k < G; k++)
+        {
+            v[i][k] = v[i][k] - mean;
+            if (c + k >= N) // (past the row's end: nothing)
+                v[i][k] = 0.0f;
+            sq[k] = v[i][k] * v[i][k];
+        }
+        q[0] = q[0] + granule_sum<G>(sq);
+    }
+    team_sum<TPR, 1>(q, scratch[1][team], j);
+    const float rstd = ln_rstd(q[0] * inv_n, eps);
+    if (!live)
+        return;
+    if (mean_out != nullptr && j == 0)
+    {
+        mean_out[row] = mean;
+        rstd_out[row] = rstd;
+    }
+    typename L::T *yr = y + row * N;
+#pragma unroll
+    for (int i = 0; i < GPT; i++)
+    {
+        const int c = (i * TPR + j) * G;
+        if (c < N)
+        {
+            float wv[G], bv[G], o[G];
+            load_param<G, PDT>(w, c, N, 1.0f, wv);
+            load_param<G, PDT>(b, c, N, 0.0f, bv);
+#pragma unroll
+            for (int k = 0; k < G; k++)
+            {
+                o[k] = v[i][k] * rstd;
+                if (w != nullptr)
+                    o[k] = o[k] * wv[k];
+                if (b != nullptr)
+                    o[k] = o[k] + bv[k];
+            }
+            L::store(yr, c, N, o);
+        }
+    }
+}
+
+// Rows too long for the registers of a workgroup: 1024 threads, three passes over the row (the second and third out of the caches).
+template <int DT, int PDT>
+__global__ __launch_bounds__(1024) void layer_norm_long_kernel(
+    const typename LowpType<DT>::T *__restrict__ x, const typename LowpType<PDT>::T *__restrict__ w,
+    const typename LowpType<PDT>::T *__restrict__ b, typename LowpType<DT>::T *__restrict__ y, float *__restrict__ mean_out,
+    float *__restrict__ rstd_out, int64_t M, int64_t N, float inv_n, float eps)
+{
+    typedef Lowp<DT> L;
+    constexpr int G = L::G, TPR = 1024;
+    __shared__ float scratch[2][TPR / 64];
+    const int j = threadIdx.x;
+    const int64_t row = blockIdx.x;
+    const typename L::T *xr = x + row * N;
+    float v[G];
+    float s[1] = {0.0f};
+    for (int64_t c = (int64_t)j * G; c < N; c += TPR * G)
+    {
+        L::load(xr, c, N, 0.0f, v);
+        s[0] = s[0] + granule_sum<G>(v);
+    }
+    team_sum<TPR, 1>(s, scratch[0], j);
+    const float mean = s[0] * inv_n;
+    float q[1] = {0.0f};
+    for (int64_t c = (int64_t)j * G; c < N; c += TPR * G)
+    {
+        L::load(xr, c, N, mean, v);
+#pragma unroll
+        for (int k = 0; k < G; k++)
+        {
+            v[k] = c + k < N ? v[k] - mean : 0.0f;
+            v[k] = v[k] * v[k];
+        }
+        q[0] = q[0] + granule_sum<G>(v);
+    }
+    team_sum<TPR, 1>(q, scratch[1], j);
+    const float rstd = ln_rstd(q[0] * inv_n, eps);
+    if (mean_out != nullptr && j == 0)
+    {
+        mean_out[row] = mean;
+        rstd_out[row] = rstd;
+    }
+    typename L::T *yr = y + row * N;
+    for (int64_t c = (int64_t)j * G; c < N; c += TPR * G)
+    {
+        float wv[G], bv[G];
+        L::load(xr, c, N, 0.0f, v);
+        load_param<G, PDT>(w, c, N, 1.0f, wv);
+        load_param<G, PDT>(b, c, N, 0.0f, bv);
+#pragma unroll
+        for (int k = 0; k < G; k++)
+        {
+            v[k] = (v[k] - mean) * rstd;
+            if (w != nullptr)
+                v[k] = v[k] * wv[k];
+            if (b != nullptr)
+                v[k] = v[k] + bv[k];
+        }
+        L::store(yr, c, N, v);
+    }
+}
+
+// ---- backward ---------------------------------------------------------------------------------
+// A workgroup owns a run of consecutive rows, its teams taking them in turn; a thread meets the same columns in every row and
+// adds up their gw and gb in registers.  At the end the teams' sums are added in order through LDS and written as one row of
+// `partial` [blocks][2][N]; layer_norm_param_kernel adds the blocks.  x and gy are read once, gx is written once.
+template <int DT, int PDT, int TPR, int E>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_grad_kernel(
+    const typename LowpType<DT>::T *__restrict__ gy, const typename LowpType<DT>::T *__restrict__ x,
+    const typename LowpType<PDT>::T *__restrict__ w, const float *__restrict__ mean_in, const float *__restrict__ rstd_in,
+    typename LowpType<DT>::T *__restrict__ gx, float *__restrict__ partial, int64_t M, int N, int64_t rows_per_block, float inv_n)
+{
+    typedef Lowp<DT> L;
+    constexpr int G = L::G, GPT = E / G;
+    constexpr int THREADS = TPR < 256 ? 256 : TPR, TEAMS = THREADS / TPR;
+    __shared__ float scratch[2][TEAMS][2 * (TPR / 64) + 1];
+    __shared__ float fold[TEAMS > 1 ? THREADS * E : 1];
+    const int tid = threadIdx.x, team = tid / TPR, j = tid % TPR;
+    const int64_t r0 = (int64_t)blockIdx.x * rows_per_block;
+    const int64_t r1 = r0 + rows_per_block < M ? r0 + rows_per_block : M;
+
+    float wv[GPT][G], aw[GPT][G], ab[GPT][G];
+#pragma unroll
+    for (int i = 0; i < GPT; i++)
+    {
+        load_param<G, PDT>(w, (int64_t)(i * TPR + j) * G, N, 1.0f, wv[i]);
+#pragma unroll
+        for (int k = 0; k < G; k++)
+            aw[i][k] = ab[i][k] = 0.0f;
+    }
+    int half = 0;
+    for (int64_t base = r0; base < r1; base += TEAMS)
+    {
+        const int64_t row = base + team;
+        const bool live = row < r1;
+        const int64_t rr = live ? row : r1 - 1;
+        float xv[GPT][G], gv[GPT][G];
+#pragma unroll
+        for (int i = 0; i < GPT; i++)
+        {
+            L::load(x + rr * N, (int64_t)(i * TPR + j) * G, N, 0.0f, xv[i]);
+            L::load(gy + rr * N, (int64_t)(i * TPR + j) * G, N, 0.0f, gv[i]);
+        }
+        const float mean = mean_in[rr], rstd = rstd_in[rr];
+        float s[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < GPT; i++)
+        {
+            const int c = (i * TPR + j) * G;
+            float g1[G], g2[G];
+#pragma unroll
+            for (int k = 0; k < G; k++)
+            {
+                xv[i][k] = (xv[i][k] - mean) * rstd;
+                if (c + k >= N) // (past the row's end, where gy came as 0)
+                    xv[i][k] = 0.0f;
+                if (live && partial != nullptr)
+                {
+                    aw[i][k] = aw[i][k] + gv[i][k] * xv[i][k];
+                    ab[i][k] = ab[i][k] + gv[i][k];
+                }
+                if (w != nullptr)
+                    gv[i][k] = gv[i][k] * wv[i][k];
+                g1[k] = gv[i][k];
+                g2[k] = gv[i][k] * xv[i][k];
+            }
+            s[0] = s[0] + granule_sum<G>(g1);
+            s[1] = s[1] + granule_sum<G>(g2);
+        }
+        if (gx == nullptr)
+            continue;
+        team_sum<TPR, 2>(s, scratch[half][team], j);
+        half ^= 1; // (the next row's sums go to the other half: a wave still reading this one is not overtaken by two rows)
+        const float m1 = s[0] * inv_n, m2 = s[1] * inv_n;
+        if (live)
+        {
+#pragma unroll
+            for (int i = 0; i < GPT; i++)
+            {
+                const int c = (i * TPR + j) * G;
+                if (c < N)
+                {
+                    float o[G];
+#pragma unroll
+                    for (int k = 0; k < G; k++)
+                        o[k] = rstd * ((gv[i][k] - m1) - xv[i][k] * m2);
+                    L::store(gx + row * N, c, N, o);
+                }
+            }
+        }
+    }
+    if (partial == nullptr)
+        return;
+    float *out = partial + (int64_t)blockIdx.x * 2 * N;
+#pragma unroll
+    for (int which = 0; which < 2; which++)
+    {
+        if (TEAMS > 1)
+        {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < GPT; i++)
+#pragma unroll
+                for (int k = 0; k < G; k++)
+                    fold[team * TPR * E + (i * TPR + j) * G + k] = which == 0 ? aw[i][k] : ab[i][k];
+            __syncthreads();
+            for (int c = tid; c < N; c += THREADS)
+            {
+                float s = fold[c];
+                for (int t = 1; t < TEAMS; t++)
+                    s = s + fold[t * TPR * E + c];
+                out[which * N + c] = s;
+            }
+        }
+        else
+        {
+#pragma unroll
+            for (int i = 0; i < GPT; i++)
+            {
+                const int c = (i * TPR + j) * G;
+                if (c < N)
+                    Lowp<REPDL_F32>::store(out + which * N, c, N, which == 0 ? aw[i] : ab[i]);
+                if (G > 4 && c + 4 < N)
+                    Lowp<REPDL_F32>::store(out + which * N, c + 4, N, (which == 0 ? aw[i] : ab[i]) + G - 4);
+            }
+        }
+    }
+}
+
+// The same for rows too long for the registers: gx by a workgroup per row that reads it twice ...
+template <int DT, int PDT>
+__global__ __launch_bounds__(1024) void layer_norm_grad_long_kernel(
+    const typename LowpType<DT>::T *__restrict__ gy, const typename LowpType<DT>::T *__restrict__ x,
+    const typename LowpType<PDT>::T *__restrict__ w, const float *__restrict__ mean_in, const float *__restrict__ rstd_in,
+    typename LowpType<DT>::T *__restrict__ gx, int64_t N, float inv_n)
+{
+    typedef Lowp<DT> L;
+    constexpr int G = L::G, TPR = 1024;
+    __shared__ float scratch[2 * (TPR / 64)];
+    const int j = threadIdx.x;
+    const int64_t row = blockIdx.x;
+    const float mean = mean_in[row], rstd = rstd_in[row];
+    float xv[G], gv[G], wv[G];
+    float s[2] = {0.0f, 0.0f};
+    for (int64_t c = (int64_t)j * G; c < N; c += TPR * G)
+    {
+        L::load(x + row * N, c, N, 0.0f, xv);
+        L::load(gy + row * N, c, N, 0.0f, gv);
+        load_param<G, PDT>(w, c, N, 1.0f, wv);
+#pragma unroll
+        for (int k = 0; k < G; k++)
+        {
+            const float xh = c + k < N ? (xv[k] - mean) * rstd : 0.0f;
+            if (w != nullptr)
+                gv[k] = gv[k] * wv[k];
+            xv[k] = gv[k] * xh;
+        }
+        s[0] = s[0] + granule_sum<G>(gv);
+        s[1] = s[1] + granule_sum<G>(xv);
+    }
+    team_sum<TPR, 2>(s, scratch, j);
+    const float m1 = s[0] * inv_n, m2 = s[1] * inv_n;
+    for (int64_t c = (int64_t)j * G; c < N; c += TPR * G)
+    {
+        L::load(x + row * N, c, N, 0.0f, xv);
+        L::load(gy + row * N, c, N, 0.0f, gv);
+        load_param<G, PDT>(w, c, N, 1.0f, wv);
+#pragma unroll
+        for (int k = 0; k < G; k++)
+        {
+            const float xh = (xv[k] - mean) * rstd;
+            if (w != nullptr)
+                gv[k] = gv[k] * wv[k];
+            gv[k] = rstd * ((gv[k] - m1) - xh * m2);
+        }
+        L::store(gx + row * N, c, N, gv);
+    }
+}
+
+// ... and the partial sums of gw and gb by a thread per granule of columns and block of rows.
+template <int DT>
+__global__ __launch_bounds__(256) void layer_norm_param_long_kernel(const typename LowpType<DT>::T *__restrict__ gy,
+                                                                    const typename LowpType<DT>::T *__restrict__ x,
+                                                                    const float *__restrict__ mean_in,
+                                                                    const float *__restrict__ rstd_in, float *__restrict__ partial,
+                                                                    int64_t M, int64_t N, int64_t rows_per_block)
+{
+    typedef Lowp<DT> L;
+    constexpr int G = L::G;
+    const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * G;
+    if (c >= N)
+        return;
+    const int64_t r0 = (int64_t)blockIdx.y * rows_per_block;
+    const int64_t r1 = r0 + rows_per_block < M ? r0 + rows_per_block : M;
+    float aw[G], ab[G];
+#pragma unroll
+    for (int k = 0; k < G; k++)
+        aw[k] = ab[k] = 0.0f;
+    for (int64_t row = r0; row < r1; row++)
+    {
+        float xv[G], gv[G];
+        L::load(x + row * N, c, N, 0.0f, xv);
+        L::load(gy + row * N, c, N, 0.0f, gv);
+        const float mean = mean_in[row], rstd = rstd_in[row];
+#pragma unroll
+        for (int k = 0; k < G; k++)
+        {
+            aw[k] = aw[k] + gv[k] * ((xv[k] - mean) * rstd);
+            ab[k] = ab[k] + gv[k];
+        }
+    }
+    float *out = partial + (int64_t)blockIdx.y * 2 * N;
+#pragma unroll
+    for (int k = 0; k < G; k++)
+        if (c + k < N)
+        {
+            out[c + k] = aw[k];
+            out[N + c + k] = ab[k];
+        }
+}
+
+// gw and gb from `blocks` rows of partial sums: 16 threads of a column add every sixteenth block, then their sums in order.
+constexpr int LN_FOLD = 16;
+template <int PDT>
+__global__ __launch_bounds__(64 * LN_FOLD) void layer_norm_param_kernel(const float *__restrict__ partial,
+                                                                        typename LowpType<PDT>::T *__restrict__ gw,
+                                                                        typename LowpType<PDT>::T *__restrict__ gb, int64_t N,
+                                                                        int blocks)
+{
+    __shared__ float sums[LN_FOLD][64];
+    const int lane = threadIdx.x & 63, part = threadIdx.x >> 6;
+    const int64_t col = (int64_t)blockIdx.x * 64 + lane;
+    float s = 0.0f;
+    if (col < 2 * N)
+    {
+#pragma unroll 8
+        for (int b = part; b < blocks; b += LN_FOLD)
+            s = s + partial[(int64_t)b * 2 * N + col];
+    }
+    sums[part][lane] = s;
+    __syncthreads();
+    if (part == 0 && col < 2 * N)
+    {
+#pragma unroll
+        for (int p = 1; p < LN_FOLD; p++)
+            s = s + sums[p][lane];
+        typename LowpType<PDT>::T *out = col < N ? gw : gb;
+        if (out != nullptr)
+            out[col < N ? col : col - N] = LowpType<PDT>::narrow(s);
+    }
+}
+
+// ---- host -------------------------------------------------------------------------------------
+template <int DT, int PDT, int TPR>
+int launch_layer_norm(const void *x, const void *w, const void *b, void *y, float *mean, float *rstd, int64_t M, int64_t N, float eps,
+                      hipStream_t s)
+{
+    typedef typename LowpType<DT>::T T;
+    typedef typename LowpType<PDT>::T P;
+    constexpr int THREADS = TPR < 256 ? 256 : TPR, TEAMS = THREADS / TPR;
+    REPDL_LAUNCH((layer_norm_kernel<DT, PDT, TPR, LN_E>), dim3((unsigned)repdl_cdiv(M, TEAMS)), dim3(THREADS), 0, s,
+                 static_cast<const T *>(x), static_cast<const P *>(w), static_cast<const P *>(b), static_cast<T *>(y), mean, rstd, M, (int)N,
+                 (float)(1.0 / (double)N), eps);
+    return repdl_launch_status();
+}
+
+template <int DT, int PDT>
+int layer_norm_typed(const void *x, const void *w, const void *b, void *y, float *mean, float *rstd, int64_t M, int64_t N, float eps,
+                     hipStream_t s)
+{
+    if (N > LN_MAX_ONCHIP)
+    {
+        typedef typename LowpType<DT>::T T;
+        typedef typename LowpType<PDT>::T P;
+        REPDL_LAUNCH((layer_norm_long_kernel<DT, PDT>), dim3((unsigned)M), dim3(1024), 0, s, static_cast<const T *>(x),
+                     static_cast<const P *>(w), static_cast<const P *>(b), static_cast<T *>(y), mean, rstd, M, N,
+                     (float)(1.0 / (double)N), eps);
+        return repdl_launch_status();
+    }
+    switch (ln_threads_per_row(N, LN_E))
+    {
+    case 4: return launch_layer_norm<DT, PDT, 4>(x, w, b, y, mean, rstd, M, N, eps, s);
+    case 8: return launch_layer_norm<DT, PDT, 8>(x, w, b, y, mean, rstd, M, N, eps, s);
+    case 16: return launch_layer_norm<DT, PDT, 16>(x, w, b, y, mean, rstd, M, N, eps, s);
+    case 32: return launch_layer_norm<DT, PDT, 32>(x, w, b, y, mean, rstd, M, N, eps, s);
+    case 64: return launch_layer_norm<DT, PDT, 64>(x, w, b, y, mean, rstd, M, N, eps, s);
+    case 128: return launch_layer_norm<DT, PDT, 128>(x, w, b, y, mean, rstd, M, N, eps, s);
+    case 256: return launch_layer_norm<DT, PDT, 256>(x, w, b, y, mean, rstd, M, N, eps, s);
+    case 512: return launch_layer_norm<DT, PDT, 512>(x, w, b, y, mean, rstd, M, N, eps, s);
+    default: return launch_layer_norm<DT, PDT, 1024>(x, w, b, y, mean, rstd, M, N, eps, s);
+    }
+}
+
+// Runs of rows of the backward pass: about 512 (two workgroups to a CU), each a multiple of the workgroup's teams.
+constexpr int64_t LN_BLOCKS = 512;
+int64_t ln_rows_per_block(int64_t M, int64_t N)
+{
+    const int tpr = N > LN_MAX_ONCHIP ? LN_MAX_TPR : ln_threads_per_row(N, LN_E);
+    const int64_t teams = tpr < 256 ? 256 / tpr : 1;
+    return repdl_cdiv(repdl_cdiv(M, LN_BLOCKS), teams) * teams;
+}
+
+template <int DT, int PDT, int TPR>
+int launch_layer_norm_grad(const void *gy, const void *x, const void *w, const float *mean, const float *rstd, void *gx, float *partial,
+                           int64_t M, int64_t N, hipStream_t s)
+{
+    typedef typename LowpType<DT>::T T;
+    typedef typename LowpType<PDT>::T P;
+    const int64_t rpb = ln_rows_per_block(M, N);
+    REPDL_LAUNCH((layer_norm_grad_kernel<DT, PDT, TPR, LN_E>), dim3((unsigned)repdl_cdiv(M, rpb)), dim3(TPR < 256 ? 256 : TPR), 0, s,
+                 static_cast<const T *>(gy), static_cast<const T *>(x), static_cast<const P *>(w), mean, rstd, static_cast<T *>(gx), partial,
+                 M, (int)N, rpb, (float)(1.0 / (double)N));
+    return repdl_launch_status();
+}
+
+template <int DT, int PDT>
+int layer_norm_grad_typed(const void *gy, const void *x, const void *w, const float *mean, const float *rstd, void *gx, float *partial,
+                          int64_t M, int64_t N, hipStream_t s)
+{
+    typedef typename LowpType<DT>::T T;
+    typedef typename LowpType<PDT>::T P;
+    if (N > LN_MAX_ONCHIP)
+    {
+        if (gx != nullptr)
+            REPDL_LAUNCH((layer_norm_grad_long_kernel<DT, PDT>), dim3((unsigned)M), dim3(1024), 0, s, static_cast<const T *>(gy),
+                         static_cast<const T *>(x), static_cast<const P *>(w), mean, rstd, static_cast<T *>(gx), N,
+                         (float)(1.0 / (double)N));
+        if (partial != nullptr)
+        {
+            const int64_t rpb = ln_rows_per_block(M, N);
+            REPDL_LAUNCH((layer_norm_param_long_kernel<DT>),
+                         dim3((unsigned)repdl_cdiv(N, 256 * Lowp<DT>::G), (unsigned)repdl_cdiv(M, rpb)), dim3(256), 0, s,
+                         static_cast<const T *>(gy), static_cast<const T *>(x), mean, rstd, partial, M, N, rpb);
+        }
+        return repdl_launch_status();
+    }
+    switch (ln_threads_per_row(N, LN_E))
+    {
+    case 4: return launch_layer_norm_grad<DT, PDT, 4>(gy, x, w, mean, rstd, gx, partial, M, N, s);
+    case 8: return launch_layer_norm_grad<DT, PDT, 8>(gy, x, w, mean, rstd, gx, partial, M, N, s);
+    case 16: return launch_layer_norm_grad<DT, PDT, 16>(gy, x, w, mean, rstd, gx, partial, M, N, s);
+    case 32: return launch_layer_norm_grad<DT, PDT, 32>(gy, x, w, mean, rstd, gx, partial, M, N, s);
+    case 64: return launch_layer_norm_grad<DT, PDT, 64>(gy, x, w, mean, rstd, gx, partial, M, N, s);
+    case 128: return launch_layer_norm_grad<DT, PDT, 128>(gy, x, w, mean, rstd, gx, partial, M, N, s);
+    case 256: return launch_layer_norm_grad<DT, PDT, 256>(gy, x, w, mean, rstd, gx, partial, M, N, s);
+    case 512: return launch_layer_norm_grad<DT, PDT, 512>(gy, x, w, mean, rstd, gx, partial, M, N, s);
+    default: return launch_layer_norm_grad<DT, PDT, 1024>(gy, x, w, mean, rstd, gx, partial, M, N, s);
+    }
+}
+
+template <int PDT>
+int layer_norm_params(const float *partial, void *gw, void *gb, int64_t M, int64_t N, hipStream_t s)
+{
+    typedef typename LowpType<PDT>::T P;
+    // (no rows: no blocks, the sums of nothing)
+    const int blocks = M == 0 ? 0 : (int)repdl_cdiv(M, ln_rows_per_block(M, N));
+    REPDL_LAUNCH((layer_norm_param_kernel<PDT>), dim3((unsigned)repdl_cdiv(2 * N, 64)), dim3(64 * LN_FOLD), 0, s, partial,
+                 static_cast<P *>(gw), static_cast<P *>(gb), N, blocks);
+    return repdl_launch_status();
+}
+
+bool ln_shape_ok(int64_t M, int64_t N, int dtype, int param_dtype)
+{
+    return M >= 0 && N >= 0 && M <= REPDL_I32_MAX && N <= REPDL_I32_MAX / 4 && repdl_known_dtype(dtype) &&
+           (param_dtype == dtype || param_dtype == REPDL_F32);
+}
+
+// f(DT, PDT) for the pairs the library has: parameters of the activation's type, or binary32
+#define LN_DISPATCH(dtype, param_dtype, f, ...)                                    \
+    ((dtype) == REPDL_F32                 ? f<REPDL_F32, REPDL_F32>(__VA_ARGS__)   \
+     : (dtype) == REPDL_BF16                                                       \
+         ? ((param_dtype) == REPDL_F32 ? f<REPDL_BF16, REPDL_F32>(__VA_ARGS__)     \
+                                       : f<REPDL_BF16, REPDL_BF16>(__VA_ARGS__))   \
+         : ((param_dtype) == REPDL_F32 ? f<REPDL_F16, REPDL_F32>(__VA_ARGS__)      \
+                                       : f<REPDL_F16, REPDL_F16>(__VA_ARGS__)))
+} // namespace
+
+REPDL_API int repdl_hip_layer_norm(const void *x, const void *weight, const void *bias, void *y, float *mean, float *rstd, int64_t M,
+                                   int64_t N, float eps, int dtype, int param_dtype, void *stream)
+{
+    REPDL_REQUIRE(ln_shape_ok(M, N, dtype, param_dtype));
+    REPDL_REQUIRE((mean == nullptr) == (rstd == nullptr));
+    if (M == 0 || N == 0)
+        return REPDL_OK;
+    REPDL_REQUIRE(x != nullptr && y != nullptr);
+    return LN_DISPATCH(dtype, param_dtype, layer_norm_typed, x, weight, bias, y, mean, rstd, M, N, eps, repdl_stream(stream));
+}
+
+REPDL_API int repdl_hip_layer_norm_grad(const void *grad_y, const void *x, const void *weight, const float *mean, const float *rstd,
+                                        void *grad_x, void *grad_weight, void *grad_bias, int64_t M, int64_t N, int dtype,
+                                        int param_dtype, void *stream)
+{
+    REPDL_REQUIRE(ln_shape_ok(M, N, dtype, param_dtype));
+    const bool params = grad_weight != nullptr || grad_bias != nullptr;
+    if (N == 0 || (grad_x == nullptr && !params) || (M == 0 && !params))
+        return REPDL_OK;
+    REPDL_REQUIRE(M == 0 || (grad_y != nullptr && x != nullptr && mean != nullptr && rstd != nullptr));
+    hipStream_t s = repdl_stream(stream);
+    float *partial = nullptr;
+    if (params && M > 0)
+    {
+        hipError_t e = repdl_ws_acquire(reinterpret_cast<void **>(&partial),
+                                        (size_t)repdl_cdiv(M, ln_rows_per_block(M, N)) * 2 * (size_t)N * sizeof(float), s);
+        if (e != hipSuccess)
+            return (int)e;
+    }
+    int rc = REPDL_OK;
+    if (M > 0)
+        rc = LN_DISPATCH(dtype, param_dtype, layer_norm_grad_typed, grad_y, x, weight, mean, rstd, grad_x, partial, M, N, s);
+    if (rc == REPDL_OK && params)
+        rc = param_dtype == REPDL_F32    ? layer_norm_params<REPDL_F32>(partial, grad_weight, grad_bias, M, N, s)
+             : param_dtype == REPDL_BF16 ? layer_norm_params<REPDL_BF16>(partial, grad_weight, grad_bias, M, N, s)
+                                         : layer_norm_params<REPDL_F16>(partial, grad_weight, grad_bias, M, N, s);
+    if (partial != nullptr)
+    {
+        const hipError_t e = repdl_ws_release(partial, s);
+        if (rc == REPDL_OK && e != hipSuccess)
+            rc = (int)e;
+    }
+    return rc;
+}
+
+REPDL_API size_t repdl_hip_layer_norm_grad_workspace_bytes(int64_t M, int64_t N)
+{
+    if (!ln_shape_ok(M, N, REPDL_F32, REPDL_F32) || M == 0 || N == 0)
+        return 0;
+    float *fake = const_cast<float *>(repdl_ws_fake_pointer(true));
+    return repdl_ws_query([&]() { return repdl_hip_layer_norm_grad(fake, fake, fake, fake, fake, fake, fake, fake, M, N, REPDL_F32, REPDL_F32, nullptr); });
+}
+
+REPDL_API int repdl_hip_layer_norm_grad_ws(const void *grad_y, const void *x, const void *weight, const float *mean, const float *rstd,
+                                           void *grad_x, void *grad_weight, void *grad_bias, int64_t M, int64_t N, int dtype,
+                                           int param_dtype, void *workspace, size_t workspace_bytes, void *stream)
+{
+    RepdlWorkspace ws(workspace, workspace_bytes);
+    return repdl_hip_layer_norm_grad(grad_y, x, weight, mean, rstd, grad_x, grad_weight, grad_bias, M, N, dtype, param_dtype, stream);
+}

@@ -1,0 +1,481 @@
+// Preference loss of paired answers, from token logits.
+//
+// Sequences 0 .. P-1 are the preferred answers, P .. 2P-1 the others; r are a reference model's log probabilities.
+//   lp_t = x[target_t] - m - log(sum_v exp(x_v - m)),  m = max_v x_v        every token whose target is not ignore_index
+//   L_i  = sum_t lp_t
+//   z_p  = beta ((L_p - L_{P+p}) - (r_p - r_{P+p}))
+//   loss = (1/P) sum_p [(1 - eps) softplus(-z_p) + eps softplus(z_p)]
+//   c_p  = d loss / d L_p = (beta / P) (eps sigma(z_p) - (1 - eps) sigma(-z_p)),  c_{P+p} = -c_p
+//   d loss / d x_{t,v} = c (1[v = target_t] - exp(x_v - m) / sum)               0 on tokens that are not counted
+//
+// Three kernels.  preference_rows_kernel reads the counted rows once and leaves (m, sum) per row and chunk of columns;
+// preference_pairs_kernel, a workgroup per pair, joins a row's chunks, adds up the sequences and makes loss and c;
+// preference_grad_kernel reads the logits again and writes the gradient.  (c of a row needs every row of its pair: the second
+// read cannot be saved.)  Both passes over the logits are bound by HBM; at 16 bits the exponentials -- crm_exp_neg, 13
+// instructions, two more for the difference and the sum and one to widen -- come to 39.3e12 / 16 = 2.4e12 elements/s,
+// 4.9 TB/s, level with it.
+//
+// The row sum is in binary32 in a fixed order (a thread's granules in turn, a butterfly over the wave, the waves, the chunks),
+// which the vocabulary and the type determine alone.  Everything per token and per pair after it is in binary64: L is a sum
+// of hundreds of terms of size ten whose differences of a tenth decide the loss.
+#include "lowp.h"
+#include "crmath.h"
+
+namespace
+{
+__device__ const uint64_t g_exp_tab3[256] = CRM_EXP_TAB_INIT;
+__device__ const float g_log_invc3[128] = CRM_LOG_INVC_INIT;
+__device__ const double g_log_hi3[128] = CRM_LOG_HI_INIT;
+__device__ const float g_log_lo3[128] = CRM_LOG_LO_INIT;
+
+struct PrefShape
+{
+    int64_t seq_stride, step_stride; // elements between sequences and between steps of the logits
+    int64_t vocab;
+    int64_t width;  // columns of a chunk
+    int64_t ignore; // target of a token that is not counted
+    int32_t steps, rows, chunks;
+};
+
+// Row of logits `row` (0 .. 2 P steps - 1)
+template <typename T>
+__device__ __forceinline__ const T *pref_row(const T *x, const PrefShape &p, uint32_t row)
+{
+    const uint32_t seq = row / (uint32_t)p.steps, step = row - seq * (uint32_t)p.steps;
+    return x + (int64_t)seq * p.seq_stride + (int64_t)step * p.step_stride;
+}
+
+// TPR threads share the E * TPR columns (at most) of one chunk of a row: 64 where a wave holds the whole row, else a workgroup.
+template <int DT, int TPR, int E>
+__global__ __launch_bounds__(256) void preference_rows_kernel(const typename LowpType<DT>::T *__restrict__ x,
+                                                              const int64_t *__restrict__ target, float2 *__restrict__ part,
+                                                              float *__restrict__ picked, int *__restrict__ counter, PrefShape p)
+{
+    typedef Lowp<DT> L;
+    constexpr int G = L::G, GPT = E / G, TEAMS = 256 / TPR;
+    __shared__ float wave_m[4], wave_s[4];
+    const int tid = threadIdx.x, j = tid % TPR;
+    if (blockIdx.x == 0 && tid == 0)
+        *counter = 0; // (of the pairs kernel, which the stream orders after this one)
+    const uint32_t item = blockIdx.x * TEAMS + tid / TPR; // (row, chunk)
+    const uint32_t row = TPR == 64 ? item : item / (uint32_t)p.chunks;
+    const uint32_t chunk = TPR == 64 ? 0 : item - row * (uint32_t)p.chunks;
+    if (row >= (uint32_t)p.rows)
+        return;
+    const int64_t t = target[row];
+    if (t == p.ignore)
+        return; // (the whole team: nothing of such a row is read or written)
+    const typename L::T *xr = pref_row(x, p, row);
+    const int64_t c0 = (int64_t)chunk * p.width;
+    const int64_t c1 = c0 + p.width < p.vocab ? c0 + p.width : p.vocab;
+    const int width = (int)(c1 - c0);
+    if (chunk == 0 && j == 0)
+        picked[row] = t >= 0 && t < p.vocab ? LowpType<DT>::widen(xr[t]) : __builtin_nanf("");
+
+    typename L::Raw raw[GPT];
+    const float none = -__builtin_inff();
+    float v[GPT][G];
+#pragma unroll
+    for (int i = 0; i < GPT; i++)
+    {
+        const int c = (i * TPR + j) * G;
+        if (c + G <= width)
+            raw[i] = L::load_raw(xr + c0 + c);
+    }
+    float m = none;
+#pragma unroll
+    for (int i = 0; i < GPT; i++)
+    {
+        const int c = (i * TPR + j) * G;
+        if (c + G <= width)
+            L::unpack(raw[i], v[i]);
+        else
+        {
+#pragma unroll
+            for (int k = 0; k < G; k++)
+                v[i][k] = c + k < width ? LowpType<DT>::widen(xr[c0 + c + k]) : none;
+        }
+#pragma unroll
+        for (int k = 0; k < G; k += 2) // (the maximum that a NaN passes through)
+            m = __builtin_elementwise_maximum(__builtin_elementwise_maximum(v[i][k], v[i][k + 1]), m);
+    }
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1)
+        m = __builtin_elementwise_maximum(m, __shfl_xor(m, off, 64));
+    if (TPR > 64)
+    {
+        if ((tid & 63) == 0)
+            wave_m[tid >> 6] = m;
+        __syncthreads();
+        m = __builtin_elementwise_maximum(__builtin_elementwise_maximum(wave_m[0], wave_m[1]),
+                                          __builtin_elementwise_maximum(wave_m[2], wave_m[3]));
+    }
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < GPT; i++)
+    {
+        if (i * TPR * G < width) // (uniform: whole rounds past the row's end)
+        {
+            float e[G];
+#pragma unroll
+            for (int k = 0; k < G; k++)
+                e[k] = crm_exp_neg(v[i][k] - m);
+#pragma unroll
+            for (int step = 1; step < G; step <<= 1)
+#pragma unroll
+                for (int k = 0; k + step < G; k += 2 * step)
+                    e[k] = e[k] + e[k + step];
+            s = s + e[0];
+        }
+    }
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1)
+        s = s + __shfl_xor(s, off, 64);
+    if (TPR > 64)
+    {
+        if ((tid & 63) == 0)
+            wave_s[tid >> 6] = s;
+        __syncthreads();
+        s = ((wave_s[0] + wave_s[1]) + wave_s[2]) + wave_s[3];
+    }
+    if (j == 0)
+        part[(int64_t)row * p.chunks + chunk] = make_float2(m, s);
+}
+
+constexpr int PAIR_THREADS = 1024;
+
+// Sum over a workgroup of one binary64 value per thread, in every thread: a butterfly per wave, the waves in order.
+__device__ __forceinline__ double pair_sum(double v, double *scratch)
+{
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1)
+        v = v + __shfl_xor(v, off, 64);
+    __syncthreads(); // (scratch may still be read by the call before)
+    if ((threadIdx.x & 63) == 0)
+        scratch[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double s = scratch[0];
+    for (int w = 1; w < PAIR_THREADS / 64; w++)
+        s = s + scratch[w];
+    return s;
+}
+
+// One pair: z -> its loss and d loss / d L of the preferred answer.  e = exp(-|z|) gives both sigmas without cancellation;
+// log(1 + e) from its series where 1 + e would round e away.  |z| is capped at 700, where every term is its limit in binary32.
+__device__ __forceinline__ void pair_terms(double z, double beta, double smoothing, double pairs, double &loss, double &coef)
+{
+    const double a = __builtin_fabs(z);
+    const double e = crm_exp64_core(a < 700.0 ? -a : -700.0, g_exp_tab3);
+    crm_log_tables lt;
+    lt.invc = g_log_invc3;
+    lt.logc_hi = g_log_hi3;
+    lt.logc_lo = g_log_lo3;
+    const double l1 = e < 0x1p-20 ? crm_fma(-0.5 * e, e, e) : crm_log64_core(1.0 + e, lt);
+    const double near = 1.0 / (1.0 + e), far = e / (1.0 + e); // sigma(|z|), sigma(-|z|)
+    const double sp = z >= 0 ? near : far, sn = z >= 0 ? far : near; // sigma(z), sigma(-z)
+    loss = (1.0 - smoothing) * (l1 + (z < 0 ? a : 0.0)) + smoothing * (l1 + (z > 0 ? a : 0.0));
+    if (smoothing == 0.0) // (0 times an infinite term is not wanted)
+        loss = l1 + (z < 0 ? a : 0.0);
+    coef = beta / pairs * (smoothing * sp - (1.0 - smoothing) * sn);
+    if (!(a == a))
+        loss = coef = a;
+}
+
+__global__ __launch_bounds__(PAIR_THREADS) void preference_pairs_kernel(const int64_t *__restrict__ target, const float2 *__restrict__ part,
+                                                                        const float *__restrict__ picked,
+                                                                        const float *__restrict__ ref, double *pair_loss, int *counter,
+                                                                        float *__restrict__ loss, float *__restrict__ logps,
+                                                                        float2 *__restrict__ row_stats, float *__restrict__ coef_out,
+                                                                        PrefShape p, int pairs, double beta, double smoothing)
+{
+    __shared__ double scratch[PAIR_THREADS / 64];
+    __shared__ int last;
+    crm_log_tables lt;
+    lt.invc = g_log_invc3;
+    lt.logc_hi = g_log_hi3;
+    lt.logc_lo = g_log_lo3;
+    const int pair = blockIdx.x;
+    double L[2];
+#pragma unroll
+    for (int side = 0; side < 2; side++)
+    {
+        const int64_t seq = side == 0 ? pair : pairs + pair;
+        double acc = 0.0;
+        for (int step = threadIdx.x; step < p.steps; step += PAIR_THREADS)
+        {
+            const int64_t row = seq * p.steps + step;
+            if (target[row] == p.ignore)
+                continue;
+            float m = -__builtin_inff(), s = 0.0f;
+            for (int c = 0; c < p.chunks; c++)
+                m = __builtin_elementwise_maximum(m, part[row * p.chunks + c].x);
+            for (int c = 0; c < p.chunks; c++)
+            {
+                const float2 v = part[row * p.chunks + c];
+                s = s + v.y * crm_exp_neg(v.x - m);
+            }
+            // s >= 1 (the maximum's own term) unless the row holds a NaN, +inf or nothing but -inf
+            const double lp = s >= 1.0f ? ((double)picked[row] - (double)m) - crm_log64_core((double)s, lt) : __builtin_nan("");
+            acc = acc + lp;
+            if (row_stats != nullptr)
+                row_stats[row] = make_float2(m, crm_div(1.0f, s));
+        }
+        L[side] = pair_sum(acc, scratch);
+    }
+    double value = 0.0, coef = 0.0;
+    if (threadIdx.x == 0)
+    {
+        double z = L[0] - L[1];
+        if (ref != nullptr)
+            z = z - ((double)ref[pair] - (double)ref[pairs + pair]);
+        pair_terms(beta * z, beta, smoothing, (double)pairs, value, coef);
+        logps[pair] = (float)L[0];
+        logps[pairs + pair] = (float)L[1];
+        if (coef_out != nullptr)
+        {
+            coef_out[pair] = (float)coef;
+            coef_out[pairs + pair] = (float)-coef;
+        }
+    }
+    if (pairs == 1)
+    {
+        if (threadIdx.x == 0)
+            *loss = (float)value;
+        return;
+    }
+    // the workgroup that ends last adds the pairs' losses, in their order
+    if (threadIdx.x == 0)
+    {
+        __hip_atomic_store(&pair_loss[pair], value, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __threadfence();
+        last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == pairs - 1;
+    }
+    __syncthreads();
+    if (!last)
+        return;
+    __threadfence();
+    double acc = 0.0;
+    for (int i = threadIdx.x; i < pairs; i += PAIR_THREADS)
+        acc = acc + __hip_atomic_load(&pair_loss[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    acc = pair_sum(acc, scratch);
+    if (threadIdx.x == 0)
+        *loss = (float)(acc / (double)pairs);
+}
+
+// d loss / d x: k e^(x - m) with k = -c / sum, and c more at the target.
+template <int DT, int TPR, int E>
+__global__ __launch_bounds__(256) void preference_grad_kernel(const typename LowpType<DT>::T *__restrict__ x,
+                                                              const int64_t *__restrict__ target,
+                                                              const float2 *__restrict__ row_stats, const float *__restrict__ coef,
+                                                              const float *__restrict__ grad_loss,
+                                                              typename LowpType<DT>::T *__restrict__ gx, PrefShape p)
+{
+    typedef Lowp<DT> L;
+    constexpr int G = L::G, GPT = E / G, TEAMS = 256 / TPR;
+    const int tid = threadIdx.x, j = tid % TPR;
+    const uint32_t item = blockIdx.x * TEAMS + tid / TPR;
+    const uint32_t row = TPR == 64 ? item : item / (uint32_t)p.chunks;
+    const uint32_t chunk = TPR == 64 ? 0 : item - row * (uint32_t)p.chunks;
+    if (row >= (uint32_t)p.rows)
+        return;
+    const int64_t c0 = (int64_t)chunk * p.width;
+    const int64_t c1 = c0 + p.width < p.vocab ? c0 + p.width : p.vocab;
+    const int width = (int)(c1 - c0);
+    typename L::T *gr = gx + (int64_t)row * p.vocab + c0;
+    const int64_t t = target[row];
+    float v[G];
+    if (t == p.ignore)
+    {
+#pragma unroll
+        for (int k = 0; k < G; k++)
+            v[k] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < GPT; i++)
+        {
+            const int c = (i * TPR + j) * G;
+            if (c < width)
+                L::store(gr, c, width, v);
+        }
+        return;
+    }
+    const typename L::T *xr = pref_row(x, p, row) + c0;
+    typename L::Raw raw[GPT];
+#pragma unroll
+    for (int i = 0; i < GPT; i++)
+    {
+        const int c = (i * TPR + j) * G;
+        if (c + G <= width)
+            raw[i] = L::load_raw(xr + c);
+    }
+    const float2 st = row_stats[row];
+    const float cc = coef[row / (uint32_t)p.steps] * *grad_loss;
+    const float k0 = -(cc * st.y);
+    const int64_t at = t - c0; // the target's column in this chunk, if it has it
+#pragma unroll
+    for (int i = 0; i < GPT; i++)
+    {
+        const int c = (i * TPR + j) * G;
+        if (c < width)
+        {
+            if (c + G <= width)
+                L::unpack(raw[i], v);
+            else
+            {
+#pragma unroll
+                for (int k = 0; k < G; k++)
+                    v[k] = c + k < width ? LowpType<DT>::widen(xr[c + k]) : 0.0f;
+            }
+#pragma unroll
+            for (int k = 0; k < G; k++)
+                v[k] = k0 * crm_exp_neg(v[k] - st.x);
+            if (at >= c && at < c + G)
+            {
+#pragma unroll
+                for (int k = 0; k < G; k++)
+                    v[k] = at == c + k ? v[k] + cc : v[k];
+            }
+            L::store(gr, c, width, v);
+        }
+    }
+}
+
+// ---- host -------------------------------------------------------------------------------------
+constexpr int PREF_E = 64, PREF_SMALL_E = 16;
+constexpr int64_t PREF_WAVE_SMALL = 64 * PREF_SMALL_E; // vocabularies that a wave holds, 16 or 64 columns a lane
+constexpr int64_t PREF_WAVE = 64 * PREF_E;
+constexpr int64_t PREF_CHUNK = 256 * PREF_E; // columns that a workgroup holds
+
+// chunks of equal width, in whole granules
+void pref_chunks(int64_t vocab, int64_t most, int32_t &chunks, int64_t &width)
+{
+    chunks = (int32_t)repdl_cdiv(vocab, most);
+    width = repdl_cdiv(repdl_cdiv(vocab, chunks), 8) * 8;
+    chunks = (int32_t)repdl_cdiv(vocab, width);
+}
+
+bool pref_shape_ok(int64_t pairs, int64_t steps, int64_t vocab, int64_t seq_stride, int64_t step_stride, int dtype)
+{
+    if (pairs < 1 || steps < 0 || vocab < 1 || seq_stride < 0 || step_stride < 0 || !repdl_known_dtype(dtype))
+        return false;
+    if (pairs > REPDL_I32_MAX / 2 || steps > REPDL_I32_MAX || vocab > REPDL_I32_MAX / 4)
+        return false;
+    return steps == 0 || (2 * pairs <= REPDL_I32_MAX / steps && 2 * pairs * steps <= REPDL_I32_MAX / (repdl_cdiv(vocab, PREF_CHUNK / 2) + 1));
+}
+
+PrefShape pref_shape(int64_t pairs, int64_t steps, int64_t vocab, int64_t seq_stride, int64_t step_stride, int64_t ignore, int64_t most)
+{
+    PrefShape p;
+    p.seq_stride = seq_stride;
+    p.step_stride = step_stride;
+    p.vocab = vocab;
+    p.ignore = ignore;
+    p.steps = (int32_t)steps;
+    p.rows = (int32_t)(2 * pairs * steps);
+    pref_chunks(vocab, most, p.chunks, p.width);
+    return p;
+}
+
+template <int DT>
+int launch_pref_rows(const void *logits, const int64_t *target, float2 *part, float *picked, int *counter, const PrefShape &p, hipStream_t s)
+{
+    const auto *x = static_cast<const typename LowpType<DT>::T *>(logits);
+    // (one workgroup at least: it clears the counter)
+    const unsigned by_wave = (unsigned)(p.rows == 0 ? 1 : repdl_cdiv(p.rows, 4));
+    const unsigned by_chunk = (unsigned)(p.rows == 0 ? 1 : (int64_t)p.rows * p.chunks);
+    if (p.vocab <= PREF_WAVE_SMALL)
+        REPDL_LAUNCH((preference_rows_kernel<DT, 64, PREF_SMALL_E>), dim3(by_wave), dim3(256), 0, s, x, target, part, picked, counter, p);
+    else if (p.vocab <= PREF_WAVE)
+        REPDL_LAUNCH((preference_rows_kernel<DT, 64, PREF_E>), dim3(by_wave), dim3(256), 0, s, x, target, part, picked, counter, p);
+    else
+        REPDL_LAUNCH((preference_rows_kernel<DT, 256, PREF_E>), dim3(by_chunk), dim3(256), 0, s, x, target, part, picked, counter, p);
+    return repdl_launch_status();
+}
+
+constexpr int PREF_GRAD_E = 32;
+
+template <int DT>
+int launch_pref_grad(const void *logits, const int64_t *target, const float2 *row_stats, const float *coef, const float *grad_loss,
+                     void *grad_logits, const PrefShape &p, hipStream_t s)
+{
+    typedef typename LowpType<DT>::T T;
+    const T *x = static_cast<const T *>(logits);
+    T *gx = static_cast<T *>(grad_logits);
+    if (p.vocab <= PREF_WAVE_SMALL)
+        REPDL_LAUNCH((preference_grad_kernel<DT, 64, PREF_SMALL_E>), dim3((unsigned)repdl_cdiv(p.rows, 4)), dim3(256), 0, s, x, target,
+                     row_stats, coef, grad_loss, gx, p);
+    else
+        REPDL_LAUNCH((preference_grad_kernel<DT, 256, PREF_GRAD_E>), dim3((unsigned)((int64_t)p.rows * p.chunks)), dim3(256), 0, s, x,
+                     target, row_stats, coef, grad_loss, gx, p);
+    return repdl_launch_status();
+}
+} // namespace
+
+REPDL_API int repdl_hip_preference_loss(const void *logits, const int64_t *target, const float *ref_logps, float *loss, float *logps,
+                                        float *row_stats, float *coef, int64_t pairs, int64_t steps, int64_t vocab, int64_t seq_stride,
+                                        int64_t step_stride, double beta, double label_smoothing, int64_t ignore_index, int dtype,
+                                        void *stream)
+{
+    REPDL_REQUIRE(pref_shape_ok(pairs, steps, vocab, seq_stride, step_stride, dtype));
+    REPDL_REQUIRE(loss != nullptr && logps != nullptr && (steps == 0 || (logits != nullptr && target != nullptr)));
+    hipStream_t s = repdl_stream(stream);
+    const PrefShape p = pref_shape(pairs, steps, vocab, seq_stride, step_stride, ignore_index, PREF_CHUNK);
+    // scratch: (m, sum) per row and chunk, the pairs' losses, the target's logit per row, a counter
+    const size_t parts = (size_t)p.rows * (size_t)p.chunks;
+    char *work = nullptr;
+    hipError_t e = repdl_ws_acquire(reinterpret_cast<void **>(&work), parts * sizeof(float2) + (size_t)pairs * sizeof(double) +
+                                                                          (size_t)p.rows * sizeof(float) + sizeof(int), s);
+    if (e != hipSuccess)
+        return (int)e;
+    float2 *part = reinterpret_cast<float2 *>(work);
+    double *pair_loss = reinterpret_cast<double *>(part + parts);
+    float *picked = reinterpret_cast<float *>(pair_loss + pairs);
+    int *counter = reinterpret_cast<int *>(picked + p.rows);
+    int rc = dtype == REPDL_F32    ? launch_pref_rows<REPDL_F32>(logits, target, part, picked, counter, p, s)
+             : dtype == REPDL_BF16 ? launch_pref_rows<REPDL_BF16>(logits, target, part, picked, counter, p, s)
+                                   : launch_pref_rows<REPDL_F16>(logits, target, part, picked, counter, p, s);
+    if (rc == REPDL_OK)
+    {
+        REPDL_LAUNCH(preference_pairs_kernel, dim3((unsigned)pairs), dim3(PAIR_THREADS), 0, s, target, part, picked, ref_logps, pair_loss,
+                     counter, loss, logps, reinterpret_cast<float2 *>(row_stats), coef, p, (int)pairs, beta, label_smoothing);
+        rc = repdl_launch_status();
+    }
+    e = repdl_ws_release(work, s);
+    return rc != REPDL_OK ? rc : (int)e;
+}
+
+REPDL_API size_t repdl_hip_preference_loss_workspace_bytes(int64_t pairs, int64_t steps, int64_t vocab)
+{
+    if (!pref_shape_ok(pairs, steps, vocab, 0, 0, REPDL_F32))
+        return 0;
+    float *fake = const_cast<float *>(repdl_ws_fake_pointer(true));
+    return repdl_ws_query([&]() {
+        return repdl_hip_preference_loss(fake, reinterpret_cast<const int64_t *>(fake), fake, fake, fake, fake, fake, pairs, steps, vocab, 0, 0,
+                                         1.0, 0.0, 0, REPDL_F32, nullptr);
+    });
+}
+
+REPDL_API int repdl_hip_preference_loss_ws(const void *logits, const int64_t *target, const float *ref_logps, float *loss, float *logps,
+                                           float *row_stats, float *coef, int64_t pairs, int64_t steps, int64_t vocab,
+                                           int64_t seq_stride, int64_t step_stride, double beta, double label_smoothing,
+                                           int64_t ignore_index, int dtype, void *workspace, size_t workspace_bytes, void *stream)
+{
+    RepdlWorkspace ws(workspace, workspace_bytes);
+    return repdl_hip_preference_loss(logits, target, ref_logps, loss, logps, row_stats, coef, pairs, steps, vocab, seq_stride, step_stride,
+                                     beta, label_smoothing, ignore_index, dtype, stream);
+}
+
+REPDL_API int repdl_hip_preference_loss_grad(const void *logits, const int64_t *target, const float *row_stats, const float *coef,
+                                             const float *grad_loss, void *grad_logits, int64_t pairs, int64_t steps, int64_t vocab,
+                                             int64_t seq_stride, int64_t step_stride, int64_t ignore_index, int dtype, void *stream)
+{
+    REPDL_REQUIRE(pref_shape_ok(pairs, steps, vocab, seq_stride, step_stride, dtype));
+    if (steps == 0)
+        return REPDL_OK;
+    REPDL_REQUIRE(logits != nullptr && target != nullptr && row_stats != nullptr && coef != nullptr && grad_loss != nullptr && grad_logits != nullptr);
+    hipStream_t s = repdl_stream(stream);
+    const PrefShape p = pref_shape(pairs, steps, vocab, seq_stride, step_stride, ignore_index, 256 * PREF_GRAD_E);
+    const float2 *stats = reinterpret_cast<const float2 *>(row_stats);
+    return dtype == REPDL_F32    ? launch_pref_grad<REPDL_F32>(logits, target, stats, coef, grad_loss, grad_logits, p, s)
+           : dtype == REPDL_BF16 ? launch_pref_grad<REPDL_BF16>(logits, target, stats, coef, grad_loss, grad_logits, p, s)
+                                 : launch_pref_grad<REPDL_F16>(logits, target, stats, coef, grad_loss, grad_logits, p, s);
+}

@@ -5,12 +5,16 @@ counterpart of RepDL's ``repdl/nn/functional.py`` (``linear``, ``conv2d``,
 ``batchnorm.py:12-66``).  Every tensor contraction, reduction, division and
 square root goes through ``repdl_amd.ops``; which operator is called, in which
 order, and which updates are in place follows the reference.
+
+``layer_norm``, ``dropout`` and ``preference_loss`` have no counterpart there: what the training
+of a language model needs beside those layers, in the same manner.
 """
 from __future__ import annotations
 
 from typing import Optional, Tuple, Union
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import func, ops
 
@@ -263,3 +267,100 @@ def batch_norm(input: torch.Tensor, running_mean: Optional[torch.Tensor], runnin
     else:
         mean, var = running_mean, running_var
     return _BatchNorm.apply(input, mean, var, weight, bias, eps)
+
+
+def _needs_grad(*tensors: Optional[torch.Tensor]) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, shape, eps):
+        y, mean, rstd = ops.layer_norm(x, shape, weight, bias, eps)
+        ctx.save_for_backward(x, weight, bias if weight is None else None, mean, rstd)  # (bias: for its type)
+        ctx.shape = shape
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        x, weight, bias, mean, rstd = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        gx, gw, gb = ops.layer_norm_grad(gy, x, mean, rstd, ctx.shape, weight, bias, need_x, need_w, need_b)
+        return gx, gw, gb, None, None
+
+
+def layer_norm(input: torch.Tensor, normalized_shape, weight: Optional[torch.Tensor] = None,
+               bias: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
+    """Layer normalisation over the trailing dimensions ``normalized_shape`` (float32, bfloat16 or float16; weight and bias
+    of the input's type or float32), with the sums of forward and backward in an order that depends on the shape and the
+    type alone: a row's result has the same bits in every batch."""
+    shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(normalized_shape)
+    if not _needs_grad(input, weight, bias):
+        return ops.layer_norm(input, shape, weight, bias, eps, stats=False)[0]
+    return _LayerNorm.apply(input, weight, bias, shape, eps)
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, p, state):
+        ctx.p, ctx.state = p, None
+        if isinstance(state, torch.Tensor):
+            ctx.save_for_backward(state)
+        else:
+            ctx.state = state
+        return ops.dropout(x, p, state, residual)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        state = ctx.saved_tensors[0] if ctx.state is None else ctx.state
+        # the mask again, from the same call of the generator
+        gx = ops.dropout(gy, ctx.p, state) if ctx.needs_input_grad[0] else None
+        return gx, gy if ctx.needs_input_grad[1] else None, None, None
+
+
+def dropout(input: torch.Tensor, p: float, state: Union[torch.Tensor, Tuple[int, int]], training: bool = True,
+            residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Dropout whose mask is a function of ``state`` = (seed, call) and the element's position (see ``ops.dropout``), the
+    same on every device, and never stored: the backward pass makes it again.  One (seed, call) is one mask: two uses that
+    are to be independent take different calls (``ops.dropout_next_call``).  With ``residual``, residual + dropout(input) in
+    one pass.  Outside training, or with p = 0, the input as it is (plus residual)."""
+    if not 0.0 <= p <= 1.0:
+        raise ValueError("dropout probability has to be between 0 and 1, but got %s" % p)
+    if not training or p == 0.0:
+        return input if residual is None else residual + input
+    if not _needs_grad(input, residual):
+        return ops.dropout(input, p, state, residual)
+    return _Dropout.apply(input, residual, p, state)
+
+
+class _Preference(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, target, ref_logps, beta, label_smoothing, ignore_index):
+        loss, logps, row_stats, coef = ops.preference_loss(logits, target, ref_logps, beta, label_smoothing, ignore_index)
+        ctx.save_for_backward(logits, target, row_stats, coef)
+        ctx.ignore_index = ignore_index
+        ctx.mark_non_differentiable(logps)
+        ctx.set_materialize_grads(False)
+        return loss, logps
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, _):
+        if g is None:
+            return (None,) * 6
+        logits, target, row_stats, coef = ctx.saved_tensors
+        return (ops.preference_loss_grad(logits, target, row_stats, coef, g, ctx.ignore_index),) + (None,) * 5
+
+
+def preference_loss(logits: torch.Tensor, target: torch.Tensor, ref_logps: Optional[torch.Tensor] = None, beta: float = 0.1,
+                    label_smoothing: float = 0.0, ignore_index: int = -100) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Preference loss of pairs of answers (see ``ops.preference_loss`` for the layout) -> (loss, log probabilities of the
+    sequences).  The loss has a gradient with respect to the logits; the log probabilities, [2 P] float32, are for the
+    record (``beta * (logps - ref_logps)`` are the implied rewards) and carry none, and ref_logps is taken as a constant."""
+    if ref_logps is not None and ref_logps.requires_grad:
+        raise NotImplementedError("preference_loss: no gradient with respect to ref_logps (detach it)")
+    if not _needs_grad(logits):
+        return ops.preference_loss(logits, target, ref_logps, beta, label_smoothing, ignore_index, grad=False)[:2]
+    return _Preference.apply(logits, target, ref_logps, beta, label_smoothing, ignore_index)

@@ -5,8 +5,11 @@ initialisation and ``state_dict`` layout are PyTorch's.
 """
 from __future__ import annotations
 
+from typing import Optional, Tuple
+
 import torch
 
+from .. import ops
 from . import functional as F
 
 
@@ -48,3 +51,49 @@ class BatchNorm1d(_BatchNorm):
 
 class BatchNorm2d(_BatchNorm):
     _check_input_dim = torch.nn.BatchNorm2d._check_input_dim
+
+
+class LayerNorm(torch.nn.LayerNorm):
+    """Layer normalisation whose rows give the same bits in every batch (no counterpart in the reference)."""
+
+    def forward(self, input: torch.Tensor) -> torch.Tensor:
+        return F.layer_norm(input, self.normalized_shape, self.weight, self.bias, self.eps)
+
+
+class Dropout(torch.nn.Dropout):
+    """Dropout whose masks are a function of the layer's seed and of how often it has been called, on any device.
+
+    ``rng_state`` (int64: seed, number of the next call) is a buffer that moves with the module and, like everything of
+    ``torch.nn.Dropout``, is not part of the state_dict: save it beside the weights to go on with the masks of an
+    interrupted run.  ``seed`` (in [0, 2^63)) defaults to a draw from PyTorch's CPU generator.  A layer that is copied
+    (``copy.deepcopy``) draws the same masks as its original: give copies that are to differ a seed of their own.
+    Recomputing a forward pass (activation checkpointing) takes another call and so another mask: use
+    ``functional.dropout`` with the state of the first one there.
+    ``forward(input, residual)`` adds the residual in the same pass."""
+
+    def __init__(self, p: float = 0.5, inplace: bool = False, seed: Optional[int] = None) -> None:
+        super().__init__(p, inplace)
+        if inplace:
+            raise NotImplementedError("Dropout: in-place is not supported")
+        if seed is None:
+            seed = int(torch.randint(0, 2 ** 63 - 1, (), dtype=torch.int64))
+        if not 0 <= seed < 2 ** 63:
+            raise ValueError("Dropout: the seed is an integer in [0, 2^63)")
+        self.register_buffer("rng_state", torch.tensor([seed, 0], dtype=torch.int64), persistent=False)
+
+    def forward(self, input: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+        if not self.training or self.p == 0.0:
+            return F.dropout(input, self.p, (0, 0), False, residual)
+        return F.dropout(input, self.p, ops.dropout_next_call(self.rng_state), True, residual)
+
+
+class PreferenceLoss(torch.nn.Module):
+    """``functional.preference_loss`` with its settings: (logits, target, ref_logps) -> (loss, log probabilities)."""
+
+    def __init__(self, beta: float = 0.1, label_smoothing: float = 0.0, ignore_index: int = -100) -> None:
+        super().__init__()
+        self.beta, self.label_smoothing, self.ignore_index = beta, label_smoothing, ignore_index
+
+    def forward(self, logits: torch.Tensor, target: torch.Tensor,
+                ref_logps: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        return F.preference_loss(logits, target, ref_logps, self.beta, self.label_smoothing, self.ignore_index)

@@ -12,7 +12,7 @@ added as public operators.
 """
 from __future__ import annotations
 
-from typing import Optional, Sequence, Union
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -150,3 +150,82 @@ def bn_gvar_term(grad_output: torch.Tensor, input: torch.Tensor, mean: torch.Ten
 def bn_gweight_term(input: torch.Tensor, mean: torch.Tensor, std: torch.Tensor, grad_output: torch.Tensor) -> torch.Tensor:
     """``((input - mean) / std) * grad_output``: the tensor that grad_weight sums (nn/batchnorm.py:60-61)."""
     return _backend(input).bn_gweight_term(input, mean, std, grad_output)
+
+
+def layer_norm(input: torch.Tensor, normalized_shape: Sequence[int], weight: Optional[torch.Tensor] = None,
+               bias: Optional[torch.Tensor] = None, eps: float = 1e-5,
+               stats: bool = True) -> Tuple[torch.Tensor, Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """The trailing dimensions ``normalized_shape`` normalised: ``(x - mean) * rstd * weight + bias``, every operation
+    rounded once in binary32, ``rstd`` the reciprocal of the square root of the biased variance plus eps.  float32,
+    bfloat16 or float16; weight and bias of that type or float32.  Returns the output and the rows' mean and rstd
+    (float32; None without ``stats``).  Not in the reference's ``ops``."""
+    return _backend(input).layer_norm(input, _row_length(input, normalized_shape), weight, bias, eps, stats)
+
+
+def layer_norm_grad(grad_output: torch.Tensor, input: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
+                    normalized_shape: Sequence[int], weight: Optional[torch.Tensor] = None, param_like: Optional[torch.Tensor] = None,
+                    need_input: bool = True, need_weight: bool = True, need_bias: bool = True):
+    """The gradients of ``layer_norm`` with respect to input, weight and bias (None where not needed), from the mean and
+    rstd it returned.  Those of weight and bias have ``normalized_shape`` and the type of weight (or of ``param_like`` where
+    there is a bias alone; float32 without either); they are sums over all rows in a fixed order."""
+    n = _row_length(input, normalized_shape)
+    gx, gw, gb = _backend(input).layer_norm_grad(grad_output, input, mean, rstd, n, weight, param_like, need_input, need_weight, need_bias)
+    shape = tuple(normalized_shape)
+    return gx, gw if gw is None else gw.view(shape), gb if gb is None else gb.view(shape)
+
+
+def _row_length(input: torch.Tensor, normalized_shape: Sequence[int]) -> int:
+    shape = tuple(normalized_shape)
+    if len(shape) == 0 or tuple(input.shape[input.dim() - len(shape):]) != shape or len(shape) > input.dim():
+        raise RuntimeError("layer_norm: the input's shape %s does not end in normalized_shape %s" % (tuple(input.shape), shape))
+    n = 1
+    for d in shape:
+        n *= d
+    return n
+
+
+def dropout(input: torch.Tensor, p: float, state: Union[torch.Tensor, Tuple[int, int]],
+            residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``input`` with each element dropped with probability p (rounded to a multiple of 2^-32) and the others scaled by
+    1 / (1 - p); with ``residual``, that plus residual in the same pass.  Which elements are dropped is a function of
+    ``state`` = (seed, call) and their position alone: word j % 4 of Philox4x32-10 at counter (j / 4, call) under the key
+    seed decides on element j of the contiguous tensor.  state: an int64 tensor of two elements on the input's device
+    (read when the kernel runs, so a captured graph follows it), or two Python integers in [0, 2^64).  The gradient
+    with respect to input is the same call on the incoming gradient.  Not in the reference's ``ops``."""
+    be = _backend(input)
+    if isinstance(state, torch.Tensor):
+        return be.dropout(input, residual, float(p), state, 0, 0)
+    seed, call = (int(v) for v in state)
+    if not (0 <= seed < 2 ** 64 and 0 <= call < 2 ** 64):
+        raise ValueError("dropout: seed and call are integers in [0, 2^64)")
+    return be.dropout(input, residual, float(p), None, seed, call)
+
+
+def dropout_next_call(state: torch.Tensor) -> torch.Tensor:
+    """A copy of the state (seed, call) of ``dropout``; ``state`` itself goes on to the next call.  One launch, on the
+    device: a graph that captures it draws a new mask at every replay."""
+    used = _backend(state).dropout_next_call(state)
+    torch.autograd.graph.increment_version(state)  # (a backward pass that still needs the old value says so)
+    return used
+
+
+def preference_loss(logits: torch.Tensor, target: torch.Tensor, ref_logps: Optional[torch.Tensor] = None, beta: float = 0.1,
+                    label_smoothing: float = 0.0, ignore_index: int = -100, grad: bool = True):
+    """Preference loss of pairs of answers from token logits.
+
+    logits [2 P, steps, vocab] (float32, bfloat16, float16; any strides between rows): sequences 0 .. P-1 are the preferred
+    answers, P .. 2P-1 the others.  target [2 P, steps] int64: the token each row predicts, ``ignore_index`` where the row is
+    not counted.  ref_logps [2 P] float32: the reference model's log probabilities (None: zeros).  With L the summed log
+    probabilities and z = beta * ((L_preferred - L_other) - (ref_preferred - ref_other)), the loss is the mean over pairs of
+    ``(1 - label_smoothing) * softplus(-z) + label_smoothing * softplus(z)``.
+    Returns (loss, L, row_stats, coef); the last two (None without ``grad``) are what ``preference_loss_grad`` takes.
+    Not in the reference's ``ops``."""
+    if not beta >= 0.0 or not 0.0 <= label_smoothing < 1.0:
+        raise ValueError("preference_loss: beta must not be negative and label_smoothing lies in [0, 1)")
+    return _backend(logits).preference_loss(logits, target, ref_logps, float(beta), float(label_smoothing), int(ignore_index), bool(grad))
+
+
+def preference_loss_grad(logits: torch.Tensor, target: torch.Tensor, row_stats: torch.Tensor, coef: torch.Tensor,
+                         grad_loss: torch.Tensor, ignore_index: int = -100) -> torch.Tensor:
+    """``grad_loss`` (0-dim) times the gradient of ``preference_loss`` with respect to the logits, contiguous, in their type."""
+    return _backend(logits).preference_loss_grad(logits, target, row_stats, coef, grad_loss, int(ignore_index))
