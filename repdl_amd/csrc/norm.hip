@@ -10,10 +10,13 @@
 // result is a function of the inputs and of the order of the sums alone.  That order is fixed by the row length, the type
 // and -- for gw and gb -- the number of rows; the device, the stream, the addresses and the other rows have no part in it.
 //
-// The two passes over a row (mean, then centred squares) read it from registers: one thread holds E = 16 or 32 of its
-// elements, as 16-byte granules TPR granules apart, TPR threads a row.  Bound: HBM.
+// The two passes over a row (mean, then centred squares) read it from registers: one thread holds E = 16 of its elements, as
+// 16-byte granules TPR granules apart, TPR threads a row.  Bound: HBM, 2 passes over the tensor forward and 3 backward.  Measured
+// (a copy of 1 GiB moves 5.1 TB/s): forward 16384 x 8192 bf16 0.096 ms = 5.6 TB/s, 8192 x 1024 f32 0.0130 = 5.2, 65536 x 256 f32
+// 0.027 = 5.0; backward with both launches 0.165 ms = 4.9 TB/s, 0.026 = 3.8, 0.048 = 4.2.
 #include "lowp.h"
 #include "crmath.h"
+#include "lanes.h"
 
 namespace
 {
@@ -26,6 +29,7 @@ __host__ __device__ constexpr int ln_threads_per_row(int64_t N, int E)
     return t;
 }
 constexpr int LN_E = 16;
+constexpr int ln_grad_threads(int tpr) { return tpr < 256 ? 256 : tpr; }
 constexpr int LN_MAX_TPR = 1024; // rows of more than LN_MAX_TPR * LN_E elements are read from memory for every pass
 constexpr int64_t LN_MAX_ONCHIP = (int64_t)LN_MAX_TPR * LN_E;
 
@@ -37,12 +41,8 @@ __device__ __forceinline__ void team_sum(float (&v)[K], float *scratch, int j)
 {
     constexpr int W = TPR < 64 ? TPR : 64;
 #pragma unroll
-    for (int off = 1; off < W; off <<= 1)
-    {
-#pragma unroll
-        for (int k = 0; k < K; k++)
-            v[k] = v[k] + __shfl_xor(v[k], off, 64);
-    }
+    for (int k = 0; k < K; k++)
+        v[k] = lanes_sum<W>(v[k]);
     if (TPR > 64)
     {
         constexpr int NW = TPR / 64;
@@ -52,7 +52,7 @@ __device__ __forceinline__ void team_sum(float (&v)[K], float *scratch, int j)
             for (int k = 0; k < K; k++)
                 scratch[k * NW + (j >> 6)] = v[k];
         }
-        __syncthreads();
+        lds_barrier();
 #pragma unroll
         for (int k = 0; k < K; k++)
         {
@@ -63,6 +63,16 @@ __device__ __forceinline__ void team_sum(float (&v)[K], float *scratch, int j)
             v[k] = s;
         }
     }
+}
+
+// A value that the whole wave shares, in scalar registers (rows of 64 threads and more: a wave works on one).
+template <int TPR>
+__device__ __forceinline__ int64_t wave_value(int64_t v)
+{
+    if (TPR < 64)
+        return v;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+    return (int64_t)(((uint64_t)hi << 32) | lo);
 }
 
 // Sum of a granule's elements: pairs, pairs of pairs.
@@ -106,7 +116,89 @@ __device__ __forceinline__ void load_param(const typename LowpType<PDT>::T *p, i
     }
 }
 
-template <int DT, int PDT, int TPR, int E>
+// The granules of one thread in a row of N elements.  The granule that would cross the row's end starts G elements before it
+// instead: all its accesses are whole 16-byte ones, its first `skip` elements are the previous granule's, computed here a second
+// time with the same result and left out of the row's sums.  A granule that lies behind the row's end repeats the last one
+// whole (skip = G) and stores nothing.  Rows shorter than a granule (TINY) are read element by element.
+template <int DT, int TPR, int E, bool TINY>
+struct RowGranules
+{
+    typedef Lowp<DT> L;
+    static constexpr int G = L::G, GPT = E / G;
+    uint32_t at[GPT];
+    int skip[GPT];
+    __device__ __forceinline__ RowGranules(int N, int j)
+    {
+#pragma unroll
+        for (int i = 0; i < GPT; i++)
+        {
+            const int c = (i * TPR + j) * G, last = TINY ? 0 : N - G;
+            at[i] = c < last ? c : last;
+            skip[i] = c - (int)at[i] < G ? c - (int)at[i] : G;
+        }
+    }
+    __device__ __forceinline__ bool stores(int i) const { return skip[i] < G; }
+    __device__ __forceinline__ typename L::Raw load(const typename L::T *row, int i, int N) const
+    {
+        if (!TINY)
+            return L::load_raw(row + at[i]);
+        typename L::Raw r = {0u, 0u, 0u, 0u};
+        typename L::T t[G];
+        __builtin_memcpy(t, &r, 16);
+#pragma unroll
+        for (int k = 0; k < G; k++)
+            if (k < N)
+                t[k] = row[k];
+        __builtin_memcpy(&r, t, 16);
+        return r;
+    }
+    __device__ __forceinline__ void store(typename L::T *row, int i, int N, const float *v) const
+    {
+        if (!TINY)
+        {
+            const typename L::Raw r = L::pack(v);
+            __builtin_memcpy(row + at[i], &r, 16);
+        }
+        else
+        {
+#pragma unroll
+            for (int k = 0; k < G; k++)
+                if (k < N)
+                    row[k] = LowpType<DT>::narrow(v[k]);
+        }
+    }
+    // what granule i adds to a sum over the row
+    __device__ __forceinline__ float sum(const float *v, int i, int N) const
+    {
+        float t[G];
+#pragma unroll
+        for (int k = 0; k < G; k++)
+            t[k] = v[k];
+        if (skip[i] > 0 || TINY)
+        {
+#pragma unroll
+            for (int k = 0; k < G; k++)
+                t[k] = k >= skip[i] && (!TINY || k < N) ? t[k] : 0.0f;
+        }
+        return granule_sum<G>(t);
+    }
+    // weight or bias at the granule's columns
+    template <int PDT>
+    __device__ __forceinline__ void param(const typename LowpType<PDT>::T *p, int i, int N, float *v) const
+    {
+        typedef Lowp<PDT> P;
+#pragma unroll
+        for (int h = 0; h < G; h += P::G)
+        {
+            if (!TINY)
+                P::unpack(P::load_raw(p + at[i] + h), v + h);
+            else
+                P::load(p, h, N, 0.0f, v + h);
+        }
+    }
+};
+
+template <int DT, int PDT, int TPR, int E, bool TINY>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_kernel(
     const typename LowpType<DT>::T *__restrict__ x, const typename LowpType<PDT>::T *__restrict__ w,
     const typename LowpType<PDT>::T *__restrict__ b, typename LowpType<DT>::T *__restrict__ y, float *__restrict__ mean_out,
@@ -117,35 +209,37 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_kernel(
     constexpr int THREADS = TPR < 256 ? 256 : TPR, TEAMS = THREADS / TPR;
     __shared__ float scratch[2][TEAMS][TPR / 64 + 1];
     const int tid = threadIdx.x, team = tid / TPR, j = tid % TPR;
-    const int64_t row = (int64_t)blockIdx.x * TEAMS + team;
+    const int64_t row = wave_value<TPR>((int64_t)blockIdx.x * TEAMS + team);
     const bool live = row < M;
     const typename L::T *xr = x + (live ? row : M - 1) * N;
+    const RowGranules<DT, TPR, E, TINY> rg(N, j);
 
-    float v[GPT][G];
+    typename L::Raw raw[GPT];
 #pragma unroll
     for (int i = 0; i < GPT; i++)
-        L::load(xr, (int64_t)(i * TPR + j) * G, N, 0.0f, v[i]);
+        raw[i] = rg.load(xr, i, N);
+    float v[GPT][G];
     float s[1] = {0.0f};
 #pragma unroll
     for (int i = 0; i < GPT; i++)
-        s[0] = s[0] + granule_sum<G>(v[i]);
+    {
+        L::unpack(raw[i], v[i]);
+        s[0] = s[0] + rg.sum(v[i], i, N);
+    }
     team_sum<TPR, 1>(s, scratch[0][team], j);
     const float mean = s[0] * inv_n;
     float q[1] = {0.0f};
 #pragma unroll
     for (int i = 0; i < GPT; i++)
     {
-        const int c = (i * TPR + j) * G;
         float sq[G];
 #pragma unroll
         for (int k = 0; k < G; k++)
         {
             v[i][k] = v[i][k] - mean;
-            if (c + k >= N) // (past the row's end: nothing)
-                v[i][k] = 0.0f;
             sq[k] = v[i][k] * v[i][k];
         }
-        q[0] = q[0] + granule_sum<G>(sq);
+        q[0] = q[0] + rg.sum(sq, i, N);
     }
     team_sum<TPR, 1>(q, scratch[1][team], j);
     const float rstd = ln_rstd(q[0] * inv_n, eps);
@@ -160,22 +254,27 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_kernel(
 #pragma unroll
     for (int i = 0; i < GPT; i++)
     {
-        const int c = (i * TPR + j) * G;
-        if (c < N)
+        if (rg.stores(i))
         {
-            float wv[G], bv[G], o[G];
-            load_param<G, PDT>(w, c, N, 1.0f, wv);
-            load_param<G, PDT>(b, c, N, 0.0f, bv);
+            float p[G];
 #pragma unroll
             for (int k = 0; k < G; k++)
+                v[i][k] = v[i][k] * rstd;
+            if (w != nullptr)
             {
-                o[k] = v[i][k] * rstd;
-                if (w != nullptr)
-                    o[k] = o[k] * wv[k];
-                if (b != nullptr)
-                    o[k] = o[k] + bv[k];
+                rg.template param<PDT>(w, i, N, p);
+#pragma unroll
+                for (int k = 0; k < G; k++)
+                    v[i][k] = v[i][k] * p[k];
             }
-            L::store(yr, c, N, o);
+            if (b != nullptr)
+            {
+                rg.template param<PDT>(b, i, N, p);
+#pragma unroll
+                for (int k = 0; k < G; k++)
+                    v[i][k] = v[i][k] + p[k];
+            }
+            rg.store(yr, i, N, v[i]);
         }
     }
 }
@@ -245,68 +344,110 @@ __global__ __launch_bounds__(1024) void layer_norm_long_kernel(
 // A workgroup owns a run of consecutive rows, its teams taking them in turn; a thread meets the same columns in every row and
 // adds up their gw and gb in registers.  At the end the teams' sums are added in order through LDS and written as one row of
 // `partial` [blocks][2][N]; layer_norm_param_kernel adds the blocks.  x and gy are read once, gx is written once.
-template <int DT, int PDT, int TPR, int E>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_grad_kernel(
+// The next row's x, gy, mean and rstd are under way while a row is worked on (two to four rows ahead changed nothing: what
+// bounds a small call is a row's latency of about a microsecond and the second launch, what bounds a large one is HBM).  A
+// workgroup's 8 waves of up to 256 registers are all that its share of a CU holds: with registers for twice the waves the loop
+// spilled and ran 10-40 % slower (8192 x 4096 bf16 0.0537 -> 0.0503 ms, 100000 x 64 0.0205 -> 0.0148).
+template <int DT, int PDT, int TPR, int E, bool TINY>
+__global__ __launch_bounds__(ln_grad_threads(TPR), TPR < 1024 ? 2 : 4) void layer_norm_grad_kernel(
     const typename LowpType<DT>::T *__restrict__ gy, const typename LowpType<DT>::T *__restrict__ x,
     const typename LowpType<PDT>::T *__restrict__ w, const float *__restrict__ mean_in, const float *__restrict__ rstd_in,
     typename LowpType<DT>::T *__restrict__ gx, float *__restrict__ partial, int64_t M, int N, int64_t rows_per_block, float inv_n)
 {
     typedef Lowp<DT> L;
     constexpr int G = L::G, GPT = E / G;
-    constexpr int THREADS = TPR < 256 ? 256 : TPR, TEAMS = THREADS / TPR;
+    constexpr int THREADS = ln_grad_threads(TPR), TEAMS = THREADS / TPR;
     __shared__ float scratch[2][TEAMS][2 * (TPR / 64) + 1];
     __shared__ float fold[TEAMS > 1 ? THREADS * E : 1];
     const int tid = threadIdx.x, team = tid / TPR, j = tid % TPR;
     const int64_t r0 = (int64_t)blockIdx.x * rows_per_block;
     const int64_t r1 = r0 + rows_per_block < M ? r0 + rows_per_block : M;
+    const RowGranules<DT, TPR, E, TINY> rg(N, j);
 
-    float wv[GPT][G], aw[GPT][G], ab[GPT][G];
+    float aw[GPT][G], ab[GPT][G];
 #pragma unroll
     for (int i = 0; i < GPT; i++)
-    {
-        load_param<G, PDT>(w, (int64_t)(i * TPR + j) * G, N, 1.0f, wv[i]);
 #pragma unroll
         for (int k = 0; k < G; k++)
             aw[i][k] = ab[i][k] = 0.0f;
+    typedef Lowp<PDT> P;
+    constexpr int WPG = G / P::G; // granules of w per granule of x
+    constexpr bool KEEP_W = !TINY && (DT != REPDL_F32 || TPR < 1024);
+    typename P::Raw wr[KEEP_W ? GPT * WPG : 1];
+    if (KEEP_W && w != nullptr)
+    {
+#pragma unroll
+        for (int i = 0; i < GPT * WPG; i++)
+            wr[i] = P::load_raw(w + rg.at[i / WPG] + i % WPG * P::G);
     }
+    typename L::Raw nx[GPT], ng[GPT];
+    float next_mean, next_rstd;
+    auto fetch = [&](int64_t at) {
+        const int64_t rr = wave_value<TPR>(at < r1 ? at : r1 - 1);
+#pragma unroll
+        for (int i = 0; i < GPT; i++)
+        {
+            nx[i] = rg.load(x + rr * N, i, N);
+            ng[i] = rg.load(gy + rr * N, i, N);
+        }
+        next_mean = mean_in[rr];
+        next_rstd = rstd_in[rr];
+    };
+    fetch(r0 + team);
     int half = 0;
     for (int64_t base = r0; base < r1; base += TEAMS)
     {
-        const int64_t row = base + team;
+        const int64_t row = wave_value<TPR>(base + team);
         const bool live = row < r1;
-        const int64_t rr = live ? row : r1 - 1;
         float xv[GPT][G], gv[GPT][G];
 #pragma unroll
         for (int i = 0; i < GPT; i++)
         {
-            L::load(x + rr * N, (int64_t)(i * TPR + j) * G, N, 0.0f, xv[i]);
-            L::load(gy + rr * N, (int64_t)(i * TPR + j) * G, N, 0.0f, gv[i]);
+            L::unpack(nx[i], xv[i]);
+            L::unpack(ng[i], gv[i]);
         }
-        const float mean = mean_in[rr], rstd = rstd_in[rr];
+        const float mean = next_mean, rstd = next_rstd;
+        if (base + TEAMS < r1)
+            fetch(row + TEAMS);
         float s[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < GPT; i++)
         {
-            const int c = (i * TPR + j) * G;
-            float g1[G], g2[G];
+            float p[G];
 #pragma unroll
             for (int k = 0; k < G; k++)
-            {
                 xv[i][k] = (xv[i][k] - mean) * rstd;
-                if (c + k >= N) // (past the row's end, where gy came as 0)
-                    xv[i][k] = 0.0f;
-                if (live && partial != nullptr)
+            if (live && partial != nullptr)
+            {
+#pragma unroll
+                for (int k = 0; k < G; k++)
                 {
                     aw[i][k] = aw[i][k] + gv[i][k] * xv[i][k];
                     ab[i][k] = ab[i][k] + gv[i][k];
                 }
-                if (w != nullptr)
-                    gv[i][k] = gv[i][k] * wv[i][k];
-                g1[k] = gv[i][k];
-                g2[k] = gv[i][k] * xv[i][k];
             }
-            s[0] = s[0] + granule_sum<G>(g1);
-            s[1] = s[1] + granule_sum<G>(g2);
+            if (w != nullptr)
+            {
+                if (KEEP_W)
+                {
+#pragma unroll
+                    for (int h = 0; h < WPG; h++)
+                    {
+                        asm("" : "+v"(wr[i * WPG + h])); // (not widened ahead of the loop: that would take twice the registers)
+                        P::unpack(wr[i * WPG + h], p + h * P::G);
+                    }
+                }
+                else
+                    rg.template param<PDT>(w, i, N, p);
+#pragma unroll
+                for (int k = 0; k < G; k++)
+                    gv[i][k] = gv[i][k] * p[k];
+            }
+#pragma unroll
+            for (int k = 0; k < G; k++)
+                p[k] = gv[i][k] * xv[i][k];
+            s[0] = s[0] + rg.sum(gv[i], i, N);
+            s[1] = s[1] + rg.sum(p, i, N);
         }
         if (gx == nullptr)
             continue;
@@ -318,14 +459,13 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_grad_kernel(
 #pragma unroll
             for (int i = 0; i < GPT; i++)
             {
-                const int c = (i * TPR + j) * G;
-                if (c < N)
+                if (rg.stores(i))
                 {
                     float o[G];
 #pragma unroll
                     for (int k = 0; k < G; k++)
                         o[k] = rstd * ((gv[i][k] - m1) - xv[i][k] * m2);
-                    L::store(gx + row * N, c, N, o);
+                    rg.store(gx + row * N, i, N, o);
                 }
             }
         }
@@ -341,9 +481,12 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_grad_kernel(
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < GPT; i++)
+                if (rg.stores(i))
+                {
 #pragma unroll
-                for (int k = 0; k < G; k++)
-                    fold[team * TPR * E + (i * TPR + j) * G + k] = which == 0 ? aw[i][k] : ab[i][k];
+                    for (int k = 0; k < G; k++)
+                        fold[team * TPR * E + rg.at[i] + k] = which == 0 ? aw[i][k] : ab[i][k];
+                }
             __syncthreads();
             for (int c = tid; c < N; c += THREADS)
             {
@@ -357,13 +500,15 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_grad_kernel(
         {
 #pragma unroll
             for (int i = 0; i < GPT; i++)
-            {
-                const int c = (i * TPR + j) * G;
-                if (c < N)
-                    Lowp<REPDL_F32>::store(out + which * N, c, N, which == 0 ? aw[i] : ab[i]);
-                if (G > 4 && c + 4 < N)
-                    Lowp<REPDL_F32>::store(out + which * N, c + 4, N, (which == 0 ? aw[i] : ab[i]) + G - 4);
-            }
+                if (rg.stores(i))
+                {
+#pragma unroll
+                    for (int h = 0; h < G; h += 4)
+                    {
+                        const Lowp<REPDL_F32>::Raw r = Lowp<REPDL_F32>::pack((which == 0 ? aw[i] : ab[i]) + h);
+                        __builtin_memcpy(out + which * N + rg.at[i] + h, &r, 16);
+                    }
+                }
         }
     }
 }
@@ -492,14 +637,14 @@ __global__ __launch_bounds__(64 * LN_FOLD) void layer_norm_param_kernel(const fl
 }
 
 // ---- host -------------------------------------------------------------------------------------
-template <int DT, int PDT, int TPR>
+template <int DT, int PDT, int TPR, bool TINY = false>
 int launch_layer_norm(const void *x, const void *w, const void *b, void *y, float *mean, float *rstd, int64_t M, int64_t N, float eps,
                       hipStream_t s)
 {
     typedef typename LowpType<DT>::T T;
     typedef typename LowpType<PDT>::T P;
     constexpr int THREADS = TPR < 256 ? 256 : TPR, TEAMS = THREADS / TPR;
-    REPDL_LAUNCH((layer_norm_kernel<DT, PDT, TPR, LN_E>), dim3((unsigned)repdl_cdiv(M, TEAMS)), dim3(THREADS), 0, s,
+    REPDL_LAUNCH((layer_norm_kernel<DT, PDT, TPR, LN_E, TINY>), dim3((unsigned)repdl_cdiv(M, TEAMS)), dim3(THREADS), 0, s,
                  static_cast<const T *>(x), static_cast<const P *>(w), static_cast<const P *>(b), static_cast<T *>(y), mean, rstd, M, (int)N,
                  (float)(1.0 / (double)N), eps);
     return repdl_launch_status();
@@ -518,6 +663,8 @@ int layer_norm_typed(const void *x, const void *w, const void *b, void *y, float
                      (float)(1.0 / (double)N), eps);
         return repdl_launch_status();
     }
+    if (N < Lowp<DT>::G)
+        return launch_layer_norm<DT, PDT, 4, true>(x, w, b, y, mean, rstd, M, N, eps, s);
     switch (ln_threads_per_row(N, LN_E))
     {
     case 4: return launch_layer_norm<DT, PDT, 4>(x, w, b, y, mean, rstd, M, N, eps, s);
@@ -532,23 +679,24 @@ int layer_norm_typed(const void *x, const void *w, const void *b, void *y, float
     }
 }
 
-// Runs of rows of the backward pass: about 512 (two workgroups to a CU), each a multiple of the workgroup's teams.
-constexpr int64_t LN_BLOCKS = 512;
+// Runs of rows of the backward pass, each a multiple of the workgroup's teams: at most two of 256 threads to a CU, one of 512 or
+// 1024.  More cost more partial sums than they hide latency (512 against 256 runs, 4096 x 16384 bf16: 0.114 -> 0.101 ms; 1024 against
+// 512, 2048 x 2048: 0.0174 -> 0.0215), fewer leave CUs idle.
 int64_t ln_rows_per_block(int64_t M, int64_t N)
 {
     const int tpr = N > LN_MAX_ONCHIP ? LN_MAX_TPR : ln_threads_per_row(N, LN_E);
-    const int64_t teams = tpr < 256 ? 256 / tpr : 1;
-    return repdl_cdiv(repdl_cdiv(M, LN_BLOCKS), teams) * teams;
+    const int64_t teams = ln_grad_threads(tpr) / tpr;
+    return repdl_cdiv(repdl_cdiv(M, tpr < 512 ? 512 : 256), teams) * teams;
 }
 
-template <int DT, int PDT, int TPR>
+template <int DT, int PDT, int TPR, bool TINY = false>
 int launch_layer_norm_grad(const void *gy, const void *x, const void *w, const float *mean, const float *rstd, void *gx, float *partial,
                            int64_t M, int64_t N, hipStream_t s)
 {
     typedef typename LowpType<DT>::T T;
     typedef typename LowpType<PDT>::T P;
     const int64_t rpb = ln_rows_per_block(M, N);
-    REPDL_LAUNCH((layer_norm_grad_kernel<DT, PDT, TPR, LN_E>), dim3((unsigned)repdl_cdiv(M, rpb)), dim3(TPR < 256 ? 256 : TPR), 0, s,
+    REPDL_LAUNCH((layer_norm_grad_kernel<DT, PDT, TPR, LN_E, TINY>), dim3((unsigned)repdl_cdiv(M, rpb)), dim3(ln_grad_threads(TPR)), 0, s,
                  static_cast<const T *>(gy), static_cast<const T *>(x), static_cast<const P *>(w), mean, rstd, static_cast<T *>(gx), partial,
                  M, (int)N, rpb, (float)(1.0 / (double)N));
     return repdl_launch_status();
@@ -575,6 +723,8 @@ int layer_norm_grad_typed(const void *gy, const void *x, const void *w, const fl
         }
         return repdl_launch_status();
     }
+    if (N < Lowp<DT>::G)
+        return launch_layer_norm_grad<DT, PDT, 4, true>(gy, x, w, mean, rstd, gx, partial, M, N, s);
     switch (ln_threads_per_row(N, LN_E))
     {
     case 4: return launch_layer_norm_grad<DT, PDT, 4>(gy, x, w, mean, rstd, gx, partial, M, N, s);
