@@ -352,3 +352,50 @@ CRM_FN float crm_exp_neg(float d)
     p = crm_fmaf(p, f, 1.0f);
     return crm_ldexpf(p, (int)n);
 }
+
+// One term of a row's sum of exponentials, without subtracting the row's maximum m first: 2^(x L - K) for L = binary32's log2(e)
+// and the integer K = rint(m L), |K| <= 2^22.  With c = 1.5 * 2^23 - K (exact), t = fma(x, L, c) has rint(x L) - K in its low bits and
+// t - c = rint(x L); f = x L - rint(x L) comes from one fused operation; the power of two is added to the exponent field of the
+// polynomial.  The caller clamps x to at least m - 86, so that no exponent field falls below 1 (what lies below is worth less than 2^-124 of
+// the maximum's term).  sum * crm_exp_base(m, K) is the sum of exp(x - m).  Degree 6 as above; degree 5 (4.9e-7 with its
+// coefficients and steps in binary32) is one instruction less where 16-bit logits make the sum bound by the vector ALU.
+// Relative error of a term: 2^-23 (5: 2^-21) + 0.224 |x - m| 2^-24 -- the product x L is not rounded.
+CRM_FN float crm_exp_term(float x, float c, int degree)
+{
+    const float t = crm_fmaf(x, 0x1.715476p+0f, c);
+    const float f = crm_fmaf(x, 0x1.715476p+0f, -(t - c));
+    float p;
+    if (degree == 5)
+    {
+        p = 0x1.23a604p-10f;
+        p = crm_fmaf(p, f, 0x1.3cbea8p-7f);
+        p = crm_fmaf(p, f, 0x1.c74322p-5f);
+        p = crm_fmaf(p, f, 0x1.ebfa4ep-3f);
+        p = crm_fmaf(p, f, 0x1.62e39ep-1f);
+    }
+    else
+    {
+        p = 0x1.470b4ap-13f;
+        p = crm_fmaf(p, f, 0x1.5f7276p-10f);
+        p = crm_fmaf(p, f, 0x1.3b270ep-7f);
+        p = crm_fmaf(p, f, 0x1.c6ae72p-5f);
+        p = crm_fmaf(p, f, 0x1.ebfbe2p-3f);
+        p = crm_fmaf(p, f, 0x1.62e432p-1f);
+    }
+    p = crm_fmaf(p, f, 1.0f);
+    return crm_u2f((crm_f2u(t) << 23) + crm_f2u(p));
+}
+
+// K and c of crm_exp_term for a maximum of at most 2^21 in magnitude, and the factor 2^(K - m L), |K - m L| <= 1/2
+CRM_FN float crm_exp_shift(float m) { return 0x1.8p23f - crm_rintf(m * 0x1.715476p+0f); }
+CRM_FN float crm_exp_base(float m, float c)
+{
+    const float g = crm_fmaf(m, 0x1.715476p+0f, c - 0x1.8p23f); // m L - K, rounded once; 2^-g by the term's own polynomial
+    float p = 0x1.470b4ap-13f;
+    p = crm_fmaf(p, -g, 0x1.5f7276p-10f);
+    p = crm_fmaf(p, -g, 0x1.3b270ep-7f);
+    p = crm_fmaf(p, -g, 0x1.c6ae72p-5f);
+    p = crm_fmaf(p, -g, 0x1.ebfbe2p-3f);
+    p = crm_fmaf(p, -g, 0x1.62e432p-1f);
+    return crm_fmaf(p, -g, 1.0f);
+}

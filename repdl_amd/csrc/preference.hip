@@ -8,18 +8,23 @@
 //   c_p  = d loss / d L_p = (beta / P) (eps sigma(z_p) - (1 - eps) sigma(-z_p)),  c_{P+p} = -c_p
 //   d loss / d x_{t,v} = c (1[v = target_t] - exp(x_v - m) / sum)               0 on tokens that are not counted
 //
-// Three kernels.  preference_rows_kernel reads the counted rows once and leaves (m, sum) per row and chunk of columns;
-// preference_pairs_kernel, a workgroup per pair, joins a row's chunks, adds up the sequences and makes loss and c;
-// preference_grad_kernel reads the logits again and writes the gradient.  (c of a row needs every row of its pair: the second
-// read cannot be saved.)  Both passes over the logits are bound by HBM; at 16 bits the exponentials -- crm_exp_neg, 13
-// instructions, two more for the difference and the sum and one to widen -- come to 39.3e12 / 16 = 2.4e12 elements/s,
-// 4.9 TB/s, level with it.
+// preference_rows_kernel reads the counted rows once and leaves (m, sum) per row and chunk of columns;
+// preference_pairs_kernel, a workgroup per pair, joins a row's chunks, adds up the sequences and makes the pair's loss and c
+// (and the last of them the mean); preference_grad_kernel reads the logits again and writes the gradient.  (c of a row needs
+// every row of its pair: the second read cannot be saved.)
+//
+// Bound: HBM, and for 16-bit logits level with it the vector ALU.  A column of the forward pass is 13 instructions -- widen, half
+// a maximum, clamp, 9 of crm_exp_term, an addition -- so 39.3e12 / 13 = 3e12 columns/s are 6 TB/s of 16-bit ones.  Measured, three
+// quarters of the tokens counted: 8192 x 131072 bf16 forward 0.295 ms = 5.45 TB/s read (0.351 with the exponential as
+// crm_exp_neg of a difference, 16 instructions; 0.275 with the hardware's exponential, whose bits are its own), backward 0.657 ms =
+// 5.7 TB/s; 8192 x 32000 f32 forward 0.135 ms = 5.8, backward 0.344 = 5.3; a pair of 12 tokens x 1000 7 + 5 us.
 //
 // The row sum is in binary32 in a fixed order (a thread's granules in turn, a butterfly over the wave, the waves, the chunks),
 // which the vocabulary and the type determine alone.  Everything per token and per pair after it is in binary64: L is a sum
 // of hundreds of terms of size ten whose differences of a tenth decide the loss.
 #include "lowp.h"
 #include "crmath.h"
+#include "lanes.h"
 
 namespace
 {
@@ -57,7 +62,7 @@ __global__ __launch_bounds__(256) void preference_rows_kernel(const typename Low
     const int tid = threadIdx.x, j = tid % TPR;
     if (blockIdx.x == 0 && tid == 0)
         *counter = 0; // (of the pairs kernel, which the stream orders after this one)
-    const uint32_t item = blockIdx.x * TEAMS + tid / TPR; // (row, chunk)
+    const uint32_t item = __builtin_amdgcn_readfirstlane(blockIdx.x * TEAMS + tid / TPR); // (row, chunk): the wave's
     const uint32_t row = TPR == 64 ? item : item / (uint32_t)p.chunks;
     const uint32_t chunk = TPR == 64 ? 0 : item - row * (uint32_t)p.chunks;
     if (row >= (uint32_t)p.rows)
@@ -99,9 +104,7 @@ __global__ __launch_bounds__(256) void preference_rows_kernel(const typename Low
         for (int k = 0; k < G; k += 2) // (the maximum that a NaN passes through)
             m = __builtin_elementwise_maximum(__builtin_elementwise_maximum(v[i][k], v[i][k + 1]), m);
     }
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1)
-        m = __builtin_elementwise_maximum(m, __shfl_xor(m, off, 64));
+    m = lanes_max<64>(m);
     if (TPR > 64)
     {
         if ((tid & 63) == 0)
@@ -110,6 +113,19 @@ __global__ __launch_bounds__(256) void preference_rows_kernel(const typename Low
         m = __builtin_elementwise_maximum(__builtin_elementwise_maximum(wave_m[0], wave_m[1]),
                                           __builtin_elementwise_maximum(wave_m[2], wave_m[3]));
     }
+    // (a maximum too large for the terms' integers, or no number: it is subtracted first)
+    float top = m;
+    if (!(__builtin_fabsf(m) <= 0x1p21f))
+    {
+#pragma unroll
+        for (int i = 0; i < GPT; i++)
+#pragma unroll
+            for (int k = 0; k < G; k++)
+                v[i][k] = v[i][k] - m;
+        top = 0.0f;
+    }
+    // (the clamp as a median of three: as a maximum it would take a second instruction that quiets NaNs)
+    const float shift = crm_exp_shift(top), least = top - 86.0f;
     float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < GPT; i++)
@@ -119,7 +135,7 @@ __global__ __launch_bounds__(256) void preference_rows_kernel(const typename Low
             float e[G];
 #pragma unroll
             for (int k = 0; k < G; k++)
-                e[k] = crm_exp_neg(v[i][k] - m);
+                e[k] = crm_exp_term(__builtin_amdgcn_fmed3f(v[i][k], least, top), shift, DT == REPDL_F32 ? 6 : 5);
 #pragma unroll
             for (int step = 1; step < G; step <<= 1)
 #pragma unroll
@@ -128,9 +144,7 @@ __global__ __launch_bounds__(256) void preference_rows_kernel(const typename Low
             s = s + e[0];
         }
     }
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1)
-        s = s + __shfl_xor(s, off, 64);
+    s = lanes_sum<64>(s);
     if (TPR > 64)
     {
         if ((tid & 63) == 0)
@@ -139,38 +153,43 @@ __global__ __launch_bounds__(256) void preference_rows_kernel(const typename Low
         s = ((wave_s[0] + wave_s[1]) + wave_s[2]) + wave_s[3];
     }
     if (j == 0)
-        part[(int64_t)row * p.chunks + chunk] = make_float2(m, s);
+        part[(int64_t)row * p.chunks + chunk] = make_float2(m, s * crm_exp_base(top, shift));
 }
 
 constexpr int PAIR_THREADS = 1024;
 
-// Sum over a workgroup of one binary64 value per thread, in every thread: a butterfly per wave, the waves in order.
-__device__ __forceinline__ double pair_sum(double v, double *scratch)
+__device__ __forceinline__ double wave_sum(double v)
 {
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1)
         v = v + __shfl_xor(v, off, 64);
-    __syncthreads(); // (scratch may still be read by the call before)
-    if ((threadIdx.x & 63) == 0)
-        scratch[threadIdx.x >> 6] = v;
-    __syncthreads();
-    double s = scratch[0];
-    for (int w = 1; w < PAIR_THREADS / 64; w++)
-        s = s + scratch[w];
-    return s;
+    return v;
 }
+
+// The tables of crm_exp64_core and crm_log64_core, in LDS.
+struct PairTables
+{
+    uint64_t exp_tab[256];
+    double log_hi[128];
+    float log_invc[128], log_lo[128];
+    __device__ crm_log_tables log_tables() const
+    {
+        crm_log_tables t;
+        t.invc = log_invc;
+        t.logc_hi = log_hi;
+        t.logc_lo = log_lo;
+        return t;
+    }
+};
 
 // One pair: z -> its loss and d loss / d L of the preferred answer.  e = exp(-|z|) gives both sigmas without cancellation;
 // log(1 + e) from its series where 1 + e would round e away.  |z| is capped at 700, where every term is its limit in binary32.
-__device__ __forceinline__ void pair_terms(double z, double beta, double smoothing, double pairs, double &loss, double &coef)
+__device__ __forceinline__ void pair_terms(double z, double beta, double smoothing, double pairs, const PairTables &tables, double &loss,
+                                           double &coef)
 {
     const double a = __builtin_fabs(z);
-    const double e = crm_exp64_core(a < 700.0 ? -a : -700.0, g_exp_tab3);
-    crm_log_tables lt;
-    lt.invc = g_log_invc3;
-    lt.logc_hi = g_log_hi3;
-    lt.logc_lo = g_log_lo3;
-    const double l1 = e < 0x1p-20 ? crm_fma(-0.5 * e, e, e) : crm_log64_core(1.0 + e, lt);
+    const double e = crm_exp64_core(a < 700.0 ? -a : -700.0, tables.exp_tab);
+    const double l1 = e < 0x1p-20 ? crm_fma(-0.5 * e, e, e) : crm_log64_core(1.0 + e, tables.log_tables());
     const double near = 1.0 / (1.0 + e), far = e / (1.0 + e); // sigma(|z|), sigma(-|z|)
     const double sp = z >= 0 ? near : far, sn = z >= 0 ? far : near; // sigma(z), sigma(-z)
     loss = (1.0 - smoothing) * (l1 + (z < 0 ? a : 0.0)) + smoothing * (l1 + (z > 0 ? a : 0.0));
@@ -190,45 +209,68 @@ __global__ __launch_bounds__(PAIR_THREADS) void preference_pairs_kernel(const in
 {
     __shared__ double scratch[PAIR_THREADS / 64];
     __shared__ int last;
-    crm_log_tables lt;
-    lt.invc = g_log_invc3;
-    lt.logc_hi = g_log_hi3;
-    lt.logc_lo = g_log_lo3;
-    const int pair = blockIdx.x;
-    double L[2];
-#pragma unroll
-    for (int side = 0; side < 2; side++)
+    __shared__ PairTables tables;
+    const int tid = threadIdx.x, pair = blockIdx.x;
+    // the first half of the workgroup takes the preferred answer's tokens, the second half the other's
+    constexpr int HALF = PAIR_THREADS / 2;
+    const int side = tid / HALF;
+    const int64_t row0 = (int64_t)(side == 0 ? pair : pairs + pair) * p.steps;
+    if (tid < 256)
+        tables.exp_tab[tid] = g_exp_tab3[tid];
+    if (tid < 128)
     {
-        const int64_t seq = side == 0 ? pair : pairs + pair;
-        double acc = 0.0;
-        for (int step = threadIdx.x; step < p.steps; step += PAIR_THREADS)
+        tables.log_hi[tid] = g_log_hi3[tid];
+        tables.log_invc[tid] = g_log_invc3[tid];
+        tables.log_lo[tid] = g_log_lo3[tid];
+    }
+    double acc = 0.0;
+    for (int base = 0; base < p.steps; base += HALF)
+    {
+        const int step = base + tid % HALF;
+        const bool live = step < p.steps;
+        const int64_t row = row0 + (live ? step : 0);
+        // (read ahead of what decides whether they count: one trip to memory instead of three)
+        const int64_t t = target[row];
+        const float x = picked[row];
+        float2 v = part[row * p.chunks];
+        float m = v.x, s = v.y;
+        for (int c = 1; c < p.chunks; c++)
         {
-            const int64_t row = seq * p.steps + step;
-            if (target[row] == p.ignore)
-                continue;
-            float m = -__builtin_inff(), s = 0.0f;
-            for (int c = 0; c < p.chunks; c++)
-                m = __builtin_elementwise_maximum(m, part[row * p.chunks + c].x);
-            for (int c = 0; c < p.chunks; c++)
-            {
-                const float2 v = part[row * p.chunks + c];
-                s = s + v.y * crm_exp_neg(v.x - m);
-            }
-            // s >= 1 (the maximum's own term) unless the row holds a NaN, +inf or nothing but -inf
-            const double lp = s >= 1.0f ? ((double)picked[row] - (double)m) - crm_log64_core((double)s, lt) : __builtin_nan("");
+            v = part[row * p.chunks + c];
+            const float top = __builtin_elementwise_maximum(m, v.x);
+            s = s * crm_exp_neg(m - top) + v.y * crm_exp_neg(v.x - top);
+            m = top;
+        }
+        if (base == 0)
+            lds_barrier(); // (the tables)
+        if (live && t != p.ignore)
+        {
+            // s >= 1 - 2^-20 (the maximum's own term is 1 but for the polynomial's error) unless the row holds a NaN, +inf or nothing but -inf
+            const double lp = s > 0.5f ? ((double)x - (double)m) - crm_log64_core((double)s, tables.log_tables()) : __builtin_nan("");
             acc = acc + lp;
             if (row_stats != nullptr)
                 row_stats[row] = make_float2(m, crm_div(1.0f, s));
         }
-        L[side] = pair_sum(acc, scratch);
     }
+    acc = wave_sum(acc);
+    if ((tid & 63) == 0)
+        scratch[tid >> 6] = acc;
+    __syncthreads();
     double value = 0.0, coef = 0.0;
-    if (threadIdx.x == 0)
+    if (tid == 0)
     {
+        double L[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+        {
+            L[i] = scratch[i * (HALF / 64)];
+            for (int w = 1; w < HALF / 64; w++)
+                L[i] = L[i] + scratch[i * (HALF / 64) + w];
+        }
         double z = L[0] - L[1];
         if (ref != nullptr)
             z = z - ((double)ref[pair] - (double)ref[pairs + pair]);
-        pair_terms(beta * z, beta, smoothing, (double)pairs, value, coef);
+        pair_terms(beta * z, beta, smoothing, (double)pairs, tables, value, coef);
         logps[pair] = (float)L[0];
         logps[pairs + pair] = (float)L[1];
         if (coef_out != nullptr)
@@ -239,32 +281,40 @@ __global__ __launch_bounds__(PAIR_THREADS) void preference_pairs_kernel(const in
     }
     if (pairs == 1)
     {
-        if (threadIdx.x == 0)
+        if (tid == 0)
             *loss = (float)value;
         return;
     }
-    // the workgroup that ends last adds the pairs' losses, in their order
-    if (threadIdx.x == 0)
+    // The workgroup that ends last adds the pairs' losses.  They and the counter are atomics of device scope, which go past the
+    // L2s of the XCDs; the wait orders a workgroup's loss before its count.  (A release fence would also write back the whole L2:
+    // 5 us here; a launch of its own for the mean takes 4.)
+    if (tid == 0)
     {
         __hip_atomic_store(&pair_loss[pair], value, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __threadfence();
-        last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == pairs - 1;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == pairs - 1;
     }
     __syncthreads();
     if (!last)
         return;
-    __threadfence();
-    double acc = 0.0;
-    for (int i = threadIdx.x; i < pairs; i += PAIR_THREADS)
+    acc = 0.0;
+    for (int i = tid; i < pairs; i += PAIR_THREADS)
         acc = acc + __hip_atomic_load(&pair_loss[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    acc = pair_sum(acc, scratch);
-    if (threadIdx.x == 0)
+    acc = wave_sum(acc);
+    if ((tid & 63) == 0) // (scratch: the first thread read the sequences' sums before the barrier above)
+        scratch[tid >> 6] = acc;
+    __syncthreads();
+    if (tid == 0)
+    {
+        for (int w = 1; w < PAIR_THREADS / 64; w++)
+            acc = acc + scratch[w];
         *loss = (float)(acc / (double)pairs);
+    }
 }
 
 // d loss / d x: k e^(x - m) with k = -c / sum, and c more at the target.
 template <int DT, int TPR, int E>
-__global__ __launch_bounds__(256) void preference_grad_kernel(const typename LowpType<DT>::T *__restrict__ x,
+__global__ __launch_bounds__(256, 4) void preference_grad_kernel(const typename LowpType<DT>::T *__restrict__ x,
                                                               const int64_t *__restrict__ target,
                                                               const float2 *__restrict__ row_stats, const float *__restrict__ coef,
                                                               const float *__restrict__ grad_loss,
@@ -273,7 +323,7 @@ __global__ __launch_bounds__(256) void preference_grad_kernel(const typename Low
     typedef Lowp<DT> L;
     constexpr int G = L::G, GPT = E / G, TEAMS = 256 / TPR;
     const int tid = threadIdx.x, j = tid % TPR;
-    const uint32_t item = blockIdx.x * TEAMS + tid / TPR;
+    const uint32_t item = __builtin_amdgcn_readfirstlane(blockIdx.x * TEAMS + tid / TPR);
     const uint32_t row = TPR == 64 ? item : item / (uint32_t)p.chunks;
     const uint32_t chunk = TPR == 64 ? 0 : item - row * (uint32_t)p.chunks;
     if (row >= (uint32_t)p.rows)
@@ -345,11 +395,12 @@ constexpr int64_t PREF_WAVE_SMALL = 64 * PREF_SMALL_E; // vocabularies that a wa
 constexpr int64_t PREF_WAVE = 64 * PREF_E;
 constexpr int64_t PREF_CHUNK = 256 * PREF_E; // columns that a workgroup holds
 
-// chunks of equal width, in whole granules
+// Chunks of about equal width, in whole rounds of a workgroup's granules (2048 columns are one of 16-bit elements, two of binary32):
+// all rounds but a row's last are full.
 void pref_chunks(int64_t vocab, int64_t most, int32_t &chunks, int64_t &width)
 {
     chunks = (int32_t)repdl_cdiv(vocab, most);
-    width = repdl_cdiv(repdl_cdiv(vocab, chunks), 8) * 8;
+    width = repdl_cdiv(repdl_cdiv(vocab, chunks), 2048) * 2048;
     chunks = (int32_t)repdl_cdiv(vocab, width);
 }
 

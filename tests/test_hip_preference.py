@@ -38,16 +38,18 @@ def check(loss, logps, grad, logits, target, ref, beta, eps, ignore=-100):
     V, P = logits.shape[2], len(L) // 2
     x = logits.detach().double().cpu()
     d = (x - x.amax(2, keepdim=True)).abs()
-    # A term exp(x - m) is off by (2 + 2.25 |d|) U (crm_exp_neg 2 + 1.25 |d|, the rounded difference |d|); weighted with the terms the
-    # |d| average to at most log V.  The sum adds at most 64 / 4 + 2 + 6 + 3 + V / 16384 roundings.  The rest of a log probability is binary64.
-    k = 2 + 2.25 * math.log(V) + 27 + V / 16384
+    # A term exp(x - m) of the sum is off by (8.2 + 0.23 |d|) U (16 bits, a polynomial of degree 5: 4.9e-7 = 8.2 U; 2 + 0.23 |d| in binary32),
+    # at most 2.25 |d| U where a large maximum is subtracted first; weighted with the terms the |d| average to at most log V.  The sum
+    # adds at most 64 / 4 + 2 + 6 + 3 + V / 16384 roundings, its factor 2^(K - m L) 2.  The rest of a log probability is binary64.
+    k = 10.2 + 2.25 * math.log(V) + 27 + V / 16384
     err_L = counted.sum(1) * k * U + 1e-12
     assert ((logps.double().cpu() - L).abs() <= err_L + L.abs() * U).all(), (logps, L)
     err_z = beta * (err_L[:P] + err_L[P:])
     assert abs(float(loss.detach()) - float(want)) <= float(err_z.mean()) + float(want) * 2 * U
     if grad is None:
         return
-    # c is off by beta/P err_z / 4 and two roundings; p by its exponential, the sum, the reciprocal and three products
+    # c is off by beta/P err_z / 4 and two roundings; p by its exponential (2 + 2.25 |d|: crm_exp_neg and the rounded difference), the
+    # sum, the reciprocal and three products
     err_c = (torch.cat([beta / P * err_z / 4] * 2)[:, None, None] + coef.abs() * 4 * U) * counted[:, :, None]
     tol = err_c * (hot - p).abs() + coef.abs() * p * (2 + 2.25 * d + k + 6) * U + coef.abs() * hot * 2 * U
     # (below the type's normal numbers a step is absolute: half of it; the exponential itself ends at 2^-149)
@@ -243,7 +245,7 @@ def test_extreme_margins():
         for eps in (0.0, 0.1):
             loss, logps = F.preference_loss(x, t, ref, 1.0, eps)
             want, _, g, (coef, _, _, _, z) = reference(x, t, ref, 1.0, eps)
-            err_z = 4 * (2 + 2.25 * math.log(10) + 27) * U  # (as in check(); exp(-z) has z's error as its relative one)
+            err_z = 4 * (10.2 + 2.25 * math.log(10) + 27) * U  # (as in check(); exp(-z) has z's error as its relative one)
             assert abs(float(loss.detach()) - float(want)) <= float(want) * (err_z + 2 * U) + 2.0 ** -149
             got = torch.autograd.grad(loss, x)[0].double().cpu()
             rel = err_z + 100 * U

@@ -69,7 +69,7 @@ def test_preference_arguments():
         assert call(**kw) == -1, kw
     need = lib.repdl_hip_preference_loss_workspace_bytes
     assert need(0, 3, 10) == 0 and need(2, 3, 0) == 0
-    assert 2 * 2 * 3 * 12 + 16 + 4 <= need(2, 3, 10) <= 2 * 2 * 3 * 12 + 16 + 4 + 512
+    assert 2 * 2 * 3 * 12 + 16 <= need(2, 3, 10) <= 2 * 2 * 3 * 12 + 16 + 512
     assert 16 * 512 * (8 * 8 + 4) <= need(8, 512, 131072) <= 16 * 512 * (8 * 8 + 4) + 1024
     assert lib.repdl_hip_preference_loss_grad(A, A, A, A, None, A, 2, 3, 10, 30, 10, -100, 0, None) == -1
     assert lib.repdl_hip_preference_loss_grad(None, None, None, None, None, None, 2, 0, 10, 30, 10, -100, 0, None) == 0
@@ -142,3 +142,51 @@ int main(void)
     subprocess.run(["gcc", "-O2", "-std=c11", "-ffp-contract=off", "-mfma", "-I", os.path.join(ROOT, "repdl_amd", "csrc"), str(src), "-o", str(exe), "-lm"], check=True)
     n, bad, worst = subprocess.run([str(exe)], check=True, stdout=subprocess.PIPE, text=True).stdout.split()
     assert int(n) > 10 ** 7 and int(bad) == 0, (n, bad, worst)
+
+
+def test_terms_of_the_row_sum_keep_their_bound(tmp_path):
+    """crm_exp_term with crm_exp_base, for maxima of every size up to 2^21 of either sign and x from m down to m - 86.  The product is
+    exp(x - m) to 2^-23 (degree 6; 2^-21 for degree 5), 0.224 |x - m| 2^-24 for binary32's log2(e), below 2^-24 for the rounding of
+    f (|f| <= 1/2 to 2^-26, times ln 2), and for the base 2^-25 ln 2 of the rounded m L - K and its polynomial's 2^-23: four 2^-24 in all
+    beside the first two terms."""
+    src = tmp_path / "exp_term.c"
+    src.write_text(r'''
+#include <stdio.h>
+#include "crmath.h"
+int main(void)
+{
+    double worst[2] = {0, 0};
+    long bad = 0, n = 0;
+    uint32_t r = 12345u;
+    for (int i = 0; i < 400000; i++)
+    {
+        r = r * 1664525u + 1013904223u;
+        const float size = ldexpf(1.0f + (float)(r >> 9) * 0x1p-23f, (int)((r >> 3) % 42u) - 21);
+        const float m = (r & 1) ? size : -size;
+        const float c = crm_exp_shift(m);
+        const double base = crm_exp_base(m, c);
+        for (int j = 0; j < 24; j++)
+        {
+            r = r * 1664525u + 1013904223u;
+            float x = j == 0 ? m : (j == 1 ? m - 86.0f : m - 86.0f * (float)(r >> 8) * 0x1p-24f);
+            if (x < m - 86.0f) x = m - 86.0f;
+            const double want = exp((double)x - (double)m);
+            for (int d = 5; d <= 6; d++)
+            {
+                const double got = (double)crm_exp_term(x, c, d) * base;
+                const double tol = want * ((d == 6 ? 0x1p-23 : 0x1p-21) + (0.25 * ((double)m - (double)x) + 4.0) * 0x1p-24);
+                const double off = fabs(got - want) / tol;
+                n++;
+                if (off > worst[d - 5]) worst[d - 5] = off;
+                if (!(off <= 1.0)) bad++;
+            }
+        }
+    }
+    printf("%ld %ld %.3f %.3f\n", n, bad, worst[0], worst[1]);
+    return 0;
+}
+''')
+    exe = tmp_path / "exp_term"
+    subprocess.run(["gcc", "-O2", "-std=c11", "-ffp-contract=off", "-mfma", "-I", os.path.join(ROOT, "repdl_amd", "csrc"), str(src), "-o", str(exe), "-lm"], check=True)
+    n, bad, w5, w6 = subprocess.run([str(exe)], check=True, stdout=subprocess.PIPE, text=True).stdout.split()
+    assert int(n) > 10 ** 7 and int(bad) == 0, (n, bad, w5, w6)
