@@ -4,7 +4,8 @@ same positional signatures, tensors in and a new tensor out, plus the elementwis
 operators (``exp``, ``log``, ``sqrt``, ``div``, ``div_scalar``) and ``mm_bias`` /
 ``conv2d_bias`` (a layer's bias added in the kernel's epilogue) and the fused elementwise
 passes of batch normalisation (``bn_apply``, ``bn_gvar_term``, ``bn_gweight_term``), layer
-normalisation, dropout and the preference loss with their gradients.
+normalisation, dropout and the preference loss with their gradients (and, as ``*_autograd``, in
+differentiable form).
 
 Two bindings of the one C-ABI library (include/repdl_hip.h) can serve it:
 
@@ -27,7 +28,7 @@ except ImportError:  # not built
 FUNCTIONS = ("mm", "conv2d", "conv2d_grad_input", "conv2d_grad_kernel", "sum1d", "sum2d_dim0", "sum2d_dim1",
              "sum4d_dim023", "softmax", "cross_entropy", "exp", "log", "sqrt", "div", "div_scalar", "mm_bias", "conv2d_bias",
              "bn_apply", "bn_gvar_term", "bn_gweight_term", "layer_norm", "layer_norm_grad", "dropout", "dropout_next_call",
-             "preference_loss", "preference_loss_grad")
+             "preference_loss", "preference_loss_grad", "layer_norm_autograd", "dropout_autograd", "preference_loss_autograd")
 if _ext_binding is not None and not all(hasattr(_ext_binding, fn) for fn in FUNCTIONS):
     import warnings
 

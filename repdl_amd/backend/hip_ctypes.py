@@ -19,6 +19,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
 
@@ -478,3 +479,70 @@ def preference_loss_grad(logits, target, row_stats, coef, grad_loss, ignore_inde
         _lib.call("repdl_hip_preference_loss_grad", _ptr(x), _ptr(t), _ptr(st), _ptr(c), _ptr(g), _ptr(out), seqs // 2, steps, vocab,
                   x.stride(0), x.stride(1), ignore_index, _DTYPES[x.dtype], _stream(x))
     return out
+
+
+# ---- autograd: the differentiable forms, as csrc/bind.cpp has them ----
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, n, weight, bias, eps):
+        y, mean, rstd = layer_norm(x, n, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, bias if weight is None else None, mean, rstd)  # (a bias alone: for its type)
+        ctx.n, ctx.shape = n, None if weight is None and bias is None else (bias if weight is None else weight).shape
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        x, weight, bias, mean, rstd = ctx.saved_tensors
+        need_x, _, need_w, need_b = ctx.needs_input_grad[:4]
+        gx, gw, gb = layer_norm_grad(gy, x, mean, rstd, ctx.n, weight, bias, need_x, need_w, need_b)
+        return gx, None, gw.view(ctx.shape) if need_w else None, gb.view(ctx.shape) if need_b else None, None
+
+
+def layer_norm_autograd(input, n: int, weight, bias, eps: float) -> torch.Tensor:
+    return _LayerNorm.apply(input, n, weight, bias, eps)
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, p, state, seed, call):
+        ctx.save_for_backward(state)
+        ctx.rest = p, seed, call
+        return dropout(x, residual, p, state, seed, call)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        p, seed, call = ctx.rest
+        # the mask again, from the same call of the generator
+        gx = dropout(gy, None, p, ctx.saved_tensors[0], seed, call) if ctx.needs_input_grad[0] else None
+        return gx, gy if ctx.needs_input_grad[1] else None, None, None, None, None
+
+
+def dropout_autograd(input, residual, p: float, state, seed: int, call: int) -> torch.Tensor:
+    return _Dropout.apply(input, residual, p, state, seed, call)
+
+
+class _Preference(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, target, ref_logps, beta, label_smoothing, ignore_index):
+        loss, logps, row_stats, coef = preference_loss(logits, target, ref_logps, beta, label_smoothing, ignore_index, True)
+        ctx.save_for_backward(logits, target, row_stats, coef)
+        ctx.ignore_index = ignore_index
+        ctx.mark_non_differentiable(logps)
+        ctx.set_materialize_grads(False)
+        return loss, logps
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, _):
+        if g is None:
+            return (None,) * 6
+        logits, target, row_stats, coef = ctx.saved_tensors
+        return (preference_loss_grad(logits, target, row_stats, coef, g, ctx.ignore_index),) + (None,) * 5
+
+
+def preference_loss_autograd(logits, target, ref_logps, beta: float, label_smoothing: float, ignore_index: int):
+    return _Preference.apply(logits, target, ref_logps, beta, label_smoothing, ignore_index)

@@ -14,7 +14,6 @@ from __future__ import annotations
 from typing import Optional, Tuple, Union
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import func, ops
 
@@ -273,23 +272,6 @@ def _needs_grad(*tensors: Optional[torch.Tensor]) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, shape, eps):
-        y, mean, rstd = ops.layer_norm(x, shape, weight, bias, eps)
-        ctx.save_for_backward(x, weight, bias if weight is None else None, mean, rstd)  # (bias: for its type)
-        ctx.shape = shape
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, gy):
-        x, weight, bias, mean, rstd = ctx.saved_tensors
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        gx, gw, gb = ops.layer_norm_grad(gy, x, mean, rstd, ctx.shape, weight, bias, need_x, need_w, need_b)
-        return gx, gw, gb, None, None
-
-
 def layer_norm(input: torch.Tensor, normalized_shape, weight: Optional[torch.Tensor] = None,
                bias: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
     """Layer normalisation over the trailing dimensions ``normalized_shape`` (float32, bfloat16 or float16; weight and bias
@@ -298,26 +280,7 @@ def layer_norm(input: torch.Tensor, normalized_shape, weight: Optional[torch.Ten
     shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(normalized_shape)
     if not _needs_grad(input, weight, bias):
         return ops.layer_norm(input, shape, weight, bias, eps, stats=False)[0]
-    return _LayerNorm.apply(input, weight, bias, shape, eps)
-
-
-class _Dropout(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, residual, p, state):
-        ctx.p, ctx.state = p, None
-        if isinstance(state, torch.Tensor):
-            ctx.save_for_backward(state)
-        else:
-            ctx.state = state
-        return ops.dropout(x, p, state, residual)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, gy):
-        state = ctx.saved_tensors[0] if ctx.state is None else ctx.state
-        # the mask again, from the same call of the generator
-        gx = ops.dropout(gy, ctx.p, state) if ctx.needs_input_grad[0] else None
-        return gx, gy if ctx.needs_input_grad[1] else None, None, None
+    return ops._backend(input).layer_norm_autograd(input, ops._row_length(input, shape), weight, bias, eps)
 
 
 def dropout(input: torch.Tensor, p: float, state: Union[torch.Tensor, Tuple[int, int]], training: bool = True,
@@ -332,26 +295,7 @@ def dropout(input: torch.Tensor, p: float, state: Union[torch.Tensor, Tuple[int,
         return input if residual is None else residual + input
     if not _needs_grad(input, residual):
         return ops.dropout(input, p, state, residual)
-    return _Dropout.apply(input, residual, p, state)
-
-
-class _Preference(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, target, ref_logps, beta, label_smoothing, ignore_index):
-        loss, logps, row_stats, coef = ops.preference_loss(logits, target, ref_logps, beta, label_smoothing, ignore_index)
-        ctx.save_for_backward(logits, target, row_stats, coef)
-        ctx.ignore_index = ignore_index
-        ctx.mark_non_differentiable(logps)
-        ctx.set_materialize_grads(False)
-        return loss, logps
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g, _):
-        if g is None:
-            return (None,) * 6
-        logits, target, row_stats, coef = ctx.saved_tensors
-        return (ops.preference_loss_grad(logits, target, row_stats, coef, g, ctx.ignore_index),) + (None,) * 5
+    return ops._backend(input).dropout_autograd(input, residual, float(p), *ops._dropout_state(state))
 
 
 def preference_loss(logits: torch.Tensor, target: torch.Tensor, ref_logps: Optional[torch.Tensor] = None, beta: float = 0.1,
@@ -363,4 +307,4 @@ def preference_loss(logits: torch.Tensor, target: torch.Tensor, ref_logps: Optio
         raise NotImplementedError("preference_loss: no gradient with respect to ref_logps (detach it)")
     if not _needs_grad(logits):
         return ops.preference_loss(logits, target, ref_logps, beta, label_smoothing, ignore_index, grad=False)[:2]
-    return _Preference.apply(logits, target, ref_logps, beta, label_smoothing, ignore_index)
+    return ops._backend(logits).preference_loss_autograd(logits, target, ref_logps, *ops._preference_settings(beta, label_smoothing, ignore_index))

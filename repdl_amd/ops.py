@@ -192,13 +192,17 @@ def dropout(input: torch.Tensor, p: float, state: Union[torch.Tensor, Tuple[int,
     seed decides on element j of the contiguous tensor.  state: an int64 tensor of two elements on the input's device
     (read when the kernel runs, so a captured graph follows it), or two Python integers in [0, 2^64).  The gradient
     with respect to input is the same call on the incoming gradient.  Not in the reference's ``ops``."""
-    be = _backend(input)
+    return _backend(input).dropout(input, residual, float(p), *_dropout_state(state))
+
+
+def _dropout_state(state: Union[torch.Tensor, Tuple[int, int]]) -> Tuple[Optional[torch.Tensor], int, int]:
+    """(tensor, 0, 0) or (None, seed, call), as the backend takes it."""
     if isinstance(state, torch.Tensor):
-        return be.dropout(input, residual, float(p), state, 0, 0)
+        return state, 0, 0
     seed, call = (int(v) for v in state)
     if not (0 <= seed < 2 ** 64 and 0 <= call < 2 ** 64):
         raise ValueError("dropout: seed and call are integers in [0, 2^64)")
-    return be.dropout(input, residual, float(p), None, seed, call)
+    return None, seed, call
 
 
 def dropout_next_call(state: torch.Tensor) -> torch.Tensor:
@@ -220,9 +224,13 @@ def preference_loss(logits: torch.Tensor, target: torch.Tensor, ref_logps: Optio
     ``(1 - label_smoothing) * softplus(-z) + label_smoothing * softplus(z)``.
     Returns (loss, L, row_stats, coef); the last two (None without ``grad``) are what ``preference_loss_grad`` takes.
     Not in the reference's ``ops``."""
+    return _backend(logits).preference_loss(logits, target, ref_logps, *_preference_settings(beta, label_smoothing, ignore_index), bool(grad))
+
+
+def _preference_settings(beta: float, label_smoothing: float, ignore_index: int) -> Tuple[float, float, int]:
     if not beta >= 0.0 or not 0.0 <= label_smoothing < 1.0:
         raise ValueError("preference_loss: beta must not be negative and label_smoothing lies in [0, 1)")
-    return _backend(logits).preference_loss(logits, target, ref_logps, float(beta), float(label_smoothing), int(ignore_index), bool(grad))
+    return float(beta), float(label_smoothing), int(ignore_index)
 
 
 def preference_loss_grad(logits: torch.Tensor, target: torch.Tensor, row_stats: torch.Tensor, coef: torch.Tensor,
