@@ -349,7 +349,8 @@ int repdl_hip_dropout_next_call(int64_t *state, int64_t *used, void *stream);
  *   logps[i] = L_i, [2 * pairs]
  * row_stats [2 * pairs, steps, 2] (8-byte aligned) and coef [2 * pairs] are what the backward pass takes (both NULL: not
  * wanted).  A target outside [0, vocab) that is not ignore_index, a NaN or +inf logit and a row of nothing but -inf make their
- * sequence's log probability, the loss and the pair's gradient NaN.
+ * sequence's log probability, the loss and the pair's gradient NaN; a target whose logit is -inf makes its sequence's log
+ * probability -inf (and the loss +inf, where that is the preferred answer).
  * preference_loss_grad: grad_logits [2 * pairs, steps, vocab], contiguous, = grad_loss[0] (device memory) * d loss / d logits;
  * +0 on rows that are not counted.  The order of every sum is a function of the extents and the type alone.
  * Scratch of the forward pass: 8 bytes per row and 16384 columns, 4 per row, 8 per pair. */

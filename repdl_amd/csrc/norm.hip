@@ -8,7 +8,11 @@
 // Every operation above is one IEEE binary32 operation (nothing is fused; the square root and the reciprocal are the
 // correctly rounded ones of crmath.h; "(1/N)" is one multiplication by float(1/N), as in the library's averages), so a
 // result is a function of the inputs and of the order of the sums alone.  That order is fixed by the row length, the type
-// and -- for gw and gb -- the number of rows; the device, the stream, the addresses and the other rows have no part in it.
+// and -- for gw and gb -- the number of rows; the device, the stream, the addresses and the other rows have no part in it:
+//   over a row   a granule's elements in pairs, pairs of pairs, ...; a thread's granules in turn; the threads of a wave as a
+//                butterfly; the waves in turn;
+//   over rows    a workgroup's run of rows, each of its teams taking every (number of teams)-th one in turn; the teams in turn; sixteen
+//                sums of every sixteenth run; those in turn.
 //
 // The two passes over a row (mean, then centred squares) read it from registers: one thread holds E = 16 of its elements, as
 // 16-byte granules TPR granules apart, TPR threads a row.  Bound: HBM, 2 passes over the tensor forward and 3 backward.  Measured

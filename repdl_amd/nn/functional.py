@@ -280,7 +280,7 @@ def layer_norm(input: torch.Tensor, normalized_shape, weight: Optional[torch.Ten
     shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(normalized_shape)
     if not _needs_grad(input, weight, bias):
         return ops.layer_norm(input, shape, weight, bias, eps, stats=False)[0]
-    return ops._backend(input).layer_norm_autograd(input, ops._row_length(input, shape), weight, bias, eps)
+    return ops._backend(input).layer_norm_autograd(input, ops._row_length(input, shape, weight, bias), weight, bias, eps)
 
 
 def dropout(input: torch.Tensor, p: float, state: Union[torch.Tensor, Tuple[int, int]], training: bool = True,

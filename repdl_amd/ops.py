@@ -159,7 +159,7 @@ def layer_norm(input: torch.Tensor, normalized_shape: Sequence[int], weight: Opt
     rounded once in binary32, ``rstd`` the reciprocal of the square root of the biased variance plus eps.  float32,
     bfloat16 or float16; weight and bias of that type or float32.  Returns the output and the rows' mean and rstd
     (float32; None without ``stats``).  Not in the reference's ``ops``."""
-    return _backend(input).layer_norm(input, _row_length(input, normalized_shape), weight, bias, eps, stats)
+    return _backend(input).layer_norm(input, _row_length(input, normalized_shape, weight, bias), weight, bias, eps, stats)
 
 
 def layer_norm_grad(grad_output: torch.Tensor, input: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
@@ -168,19 +168,22 @@ def layer_norm_grad(grad_output: torch.Tensor, input: torch.Tensor, mean: torch.
     """The gradients of ``layer_norm`` with respect to input, weight and bias (None where not needed), from the mean and
     rstd it returned.  Those of weight and bias have ``normalized_shape`` and the type of weight (or of ``param_like`` where
     there is a bias alone; float32 without either); they are sums over all rows in a fixed order."""
-    n = _row_length(input, normalized_shape)
+    n = _row_length(input, normalized_shape, weight, param_like)
     gx, gw, gb = _backend(input).layer_norm_grad(grad_output, input, mean, rstd, n, weight, param_like, need_input, need_weight, need_bias)
     shape = tuple(normalized_shape)
     return gx, gw if gw is None else gw.view(shape), gb if gb is None else gb.view(shape)
 
 
-def _row_length(input: torch.Tensor, normalized_shape: Sequence[int]) -> int:
+def _row_length(input: torch.Tensor, normalized_shape: Sequence[int], *params: Optional[torch.Tensor]) -> int:
     shape = tuple(normalized_shape)
-    if len(shape) == 0 or tuple(input.shape[input.dim() - len(shape):]) != shape or len(shape) > input.dim():
+    if len(shape) == 0 or len(shape) > input.dim() or tuple(input.shape[input.dim() - len(shape):]) != shape:
         raise RuntimeError("layer_norm: the input's shape %s does not end in normalized_shape %s" % (tuple(input.shape), shape))
     n = 1
     for d in shape:
         n *= d
+    for p in params:
+        if p is not None and tuple(p.shape) != shape:
+            raise RuntimeError("layer_norm: a weight or bias of shape %s for normalized_shape %s" % (tuple(p.shape), shape))
     return n
 
 

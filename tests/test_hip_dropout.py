@@ -184,6 +184,17 @@ def test_side_stream_and_both_bindings():
     assert hip_ctypes.dropout_next_call(state).tolist() == [1, 1] and state.tolist() == [1, 2]
 
 
+def test_more_elements_than_32_bits_count():
+    from repdl_amd import ops
+
+    n = (1 << 32) + 4099                              # (in 16 bits; block numbers past 2^30, element numbers past 2^32)
+    x = torch.ones(n, dtype=torch.bfloat16, device="cuda")
+    y = ops.dropout(x, 0.5, (12, 34))
+    for first, count in ((0, 1000), ((1 << 31) - 512, 1024), ((1 << 32) - 512, 4611)):
+        keep = torch.from_numpy(philox.words(count, 12, 34, first).astype(np.int64)) >= 1 << 31
+        assert torch.equal(y[first:first + count].cpu() != 0, keep)
+
+
 def test_refusals():
     from repdl_amd import ops
     from repdl_amd.nn import functional as F

@@ -46,6 +46,19 @@ def test_only_the_wanted_gradients(binding, wanted):
         assert (t.grad is not None) == t.requires_grad and (t.grad is None or torch.equal(t.grad, g))
 
 
+def test_a_bias_alone(binding):
+    from repdl_amd.nn import functional as F
+
+    x = gen.normal_like(8, 6, 4, 10).to(torch.bfloat16).cuda()
+    b = gen.normal_like(9, 4, 10).to(torch.bfloat16).cuda().requires_grad_()
+    gy = gen.normal_like(10, 6, 4, 10).to(torch.bfloat16).cuda()
+    F.layer_norm(x, (4, 10), None, b).backward(gy)
+    assert b.grad.shape == b.shape and b.grad.dtype == b.dtype
+    # (six terms: at most 6 + 48 roundings of the sum of magnitudes, and the one to bfloat16)
+    want = gy.double().sum(0)
+    assert ((b.grad.double() - want).abs() <= gy.double().abs().sum(0) * 54 * 2.0 ** -24 + want.abs() * 2.0 ** -8).all()
+
+
 def test_residual_of_dropout_alone(binding):
     from repdl_amd.nn import functional as F
 

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import gen
+import norm_model
 
 pytestmark = pytest.mark.gpu
 
@@ -232,17 +233,72 @@ def test_empty_and_special_rows():
 
 def test_refusals():
     from repdl_amd import ops
+    from repdl_amd.nn import functional as F
 
     x = torch.zeros(4, 8, device="cuda")
     ok = torch.ones(8, device="cuda")
     bad = [lambda: ops.layer_norm(x.cpu(), (8,)), lambda: ops.layer_norm(x.double(), (8,)), lambda: ops.layer_norm(x, (4,)),
            lambda: ops.layer_norm(x, ()), lambda: ops.layer_norm(x, (4, 8, 1)), lambda: ops.layer_norm(x, (8,), ok[:7]),
            lambda: ops.layer_norm(x, (8,), ok.half()), lambda: ops.layer_norm(x.half(), (8,), ok, ok.half()),
-           lambda: ops.layer_norm(x, (8,), ok.cpu()), lambda: ops.layer_norm_grad(x, x, ok[:3], ok[:4], (8,)),
+           lambda: ops.layer_norm(x, (8,), ok.cpu()), lambda: ops.layer_norm(x, (8,), ok.view(2, 4)), lambda: F.layer_norm(x, 8, ok.view(1, 8).requires_grad_()), lambda: ops.layer_norm_grad(x, x, ok[:3], ok[:4], (8,)),
            lambda: ops.layer_norm_grad(x.half(), x, ok[:4], ok[:4], (8,)), lambda: ops.layer_norm_grad(x[:3], x, ok[:4], ok[:4], (8,))]
     for call in bad:
         with pytest.raises(RuntimeError):
             call()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(1, 1), (70, 3), (300, 7), (5, 8), (600, 20), (2000, 63), (37, 64), (1300, 100), (700, 1000), (40, 1025), (9, 2048), (600, 4100),
+                                   (5, 8191), (300, 16384)], ids=str)
+def test_bits_of_the_documented_order(shape, kind):
+    """Outputs, statistics and all three gradients against a model of the sums' order in numpy's binary32: every bit."""
+    from repdl_amd import ops
+
+    t = TYPES[kind]
+    x, w, b, gy = data(*shape, t, t, seed=110)
+    y, mean, rstd = ops.layer_norm(x, shape[1:], w, b)
+    gx, gw, gb = ops.layer_norm_grad(gy, x, mean, rstd, shape[1:], w)
+    model = norm_model.LayerNorm(*shape, granule=4 if kind == "f32" else 8)
+    args = [v.float().cpu().numpy() for v in (x, w, b, gy)]
+    want_y, want_mean, want_rstd, xh = model.forward(args[0], args[1], args[2], 1e-5)
+    want_gx, want_gw, want_gb = model.backward(args[3], xh, want_rstd, args[1])
+    for got, want in ((mean, want_mean), (rstd, want_rstd), (y, want_y), (gx, want_gx), (gw, want_gw), (gb, want_gb)):
+        assert torch.equal(got.cpu(), torch.from_numpy(want).to(got.dtype))
+
+
+def test_more_elements_than_32_bits_count():
+    from repdl_amd import ops
+
+    rows, cols = (1 << 19) + 3, 4096 + 8           # 2.15e9 elements
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device="cuda")
+    part = gen.normal_like(120, 64, cols).to(torch.bfloat16).cuda()
+    x.copy_(part[:1].expand(rows, cols))
+    x[-64:] = part
+    w, b = gen.normal_like(121, cols).cuda(), gen.normal_like(122, cols).cuda()
+    y, mean, rstd = ops.layer_norm(x, (cols,), w, b)
+    want = ops.layer_norm(part, (cols,), w, b)
+    assert torch.equal(y[-64:], want[0]) and torch.equal(mean[-64:], want[1]) and torch.equal(y[:1], want[0][:1])
+    gx, gw, gb = ops.layer_norm_grad(x, x, mean, rstd, (cols,), w)  # (the rows as their own incoming gradient)
+    assert torch.equal(gx[-64:], ops.layer_norm_grad(part, part, want[1], want[2], (cols,), w)[0])
+    exact = part.double().sum(0) + part[0].double() * (rows - 64)
+    terms = part.double().abs().sum(0) + part[0].double().abs() * (rows - 64)
+    # runs of 2050 rows in turn, then 32 + 16 partial sums: at most 2100 roundings, each of at most U of the sum of magnitudes
+    assert ((gb.double() - exact).abs() <= 2100 * U * terms).all()
+
+
+def test_entry_points_with_the_librarys_scratch():
+    """The C entry point that brings its own scratch gives the bits of the one that is handed some."""
+    import ctypes
+
+    from repdl_amd import _lib, ops
+
+    x, w, b, gy = data(500, 300, torch.float32, torch.float32, seed=130)
+    _, mean, rstd = ops.layer_norm(x, (300,), w, b)
+    want = ops.layer_norm_grad(gy, x, mean, rstd, (300,), w)
+    got = [torch.empty_like(t) for t in want]
+    p = [ctypes.c_void_p(t.data_ptr()) for t in (gy, x, w, mean, rstd, *got)]
+    _lib.call("repdl_hip_layer_norm_grad", *p, 500, 300, 0, 0, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+    assert all(torch.equal(g, v) for g, v in zip(got, want))
 
 
 def test_side_stream_and_graph():

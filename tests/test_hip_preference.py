@@ -169,10 +169,10 @@ def test_tokens_that_are_not_counted_are_not_read():
     assert torch.equal(logps3, F.preference_loss(junk, w, ref)[1])
     nothing = torch.full_like(t, -100)
     loss4, logps4 = F.preference_loss(junk, nothing)
-    assert not logps4.any() and float(loss4) == pytest.approx(math.log(2), rel=2 * U)
+    assert not logps4.any() and float(loss4.detach()) == pytest.approx(math.log(2), rel=2 * U)
     assert not torch.autograd.grad(loss4, junk)[0].any()
     loss5, logps5 = F.preference_loss(x[:, :0], t[:, :0])  # no steps at all
-    assert not logps5.any() and float(loss5) == float(loss4)
+    assert not logps5.any() and float(loss5.detach()) == float(loss4.detach())
     (g5,) = torch.autograd.grad(F.preference_loss(x[:, :0], t[:, :0])[0], x)
     assert not g5.any()
 
@@ -262,6 +262,40 @@ def test_many_pairs_in_order():
     for _ in range(5):
         again = ops.preference_loss(x, t, ref)
         assert torch.equal(again[0], loss) and torch.equal(again[1], logps)
+
+
+def test_more_elements_than_32_bits_count():
+    from repdl_amd import ops
+
+    P, S, V = 2, 8200, 65536 + 3                      # 2.15e9 elements
+    x = torch.zeros(2 * P, S, V, dtype=torch.bfloat16, device="cuda")
+    tail = gen.normal_like(86, 8, V).to(torch.bfloat16).cuda()
+    x[-1, -8:] = tail
+    t = torch.full((2 * P, S), -100, device="cuda")
+    t[-1, -8:] = gen.labels(87, 8, V).cuda()
+    loss, logps, stats, coef = ops.preference_loss(x, t)
+    g = ops.preference_loss_grad(x, t, stats, coef, torch.ones((), device="cuda"))
+    small, ts = x[:, -8:].clone(), t[:, -8:].clone()  # the same tokens alone
+    loss2, logps2, stats2, coef2 = ops.preference_loss(small, ts)
+    assert torch.equal(loss, loss2) and torch.equal(logps, logps2)
+    assert torch.equal(g[:, -8:], ops.preference_loss_grad(small, ts, stats2, coef2, torch.ones((), device="cuda")))
+    assert not g[:, :-8].any()
+
+
+def test_entry_point_with_the_librarys_scratch():
+    """The C entry point that brings its own scratch gives the bits of the one that is handed some."""
+    import ctypes
+
+    from repdl_amd import _lib, ops
+
+    x, t, ref = data(2, 5, 9000, "f32", seed=88)
+    want = ops.preference_loss(x, t, ref, 0.1, 0.1)
+    got = [torch.zeros_like(v) for v in want]
+    p = lambda v: ctypes.c_void_p(v.data_ptr())  # noqa: E731
+    _lib.call("repdl_hip_preference_loss", p(x), p(t), p(ref), *(p(v) for v in got), 2, 5, 9000, 5 * 9000, 9000, 0.1, 0.1, -100, 0,
+              ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(got[3], want[3])
+    assert torch.equal(got[2][t != -100], want[2][t != -100])
 
 
 def test_side_stream_and_graph():
