@@ -13,7 +13,8 @@
 //
 // Bound: HBM, 8 B per element in binary32 (12 with a residual), 4 (6) in 16 bits.  The ten rounds are 20 products of 32 by 32
 // to 64 bits (a quarter of the vector rate each) and about 20 three-operand exclusive ors for four elements, 25 issue slots per
-// element: 39.3e12 / 25 = 1.6e12 elements/s, which at 16 bits is 6.3 TB/s, just above the copy rate.
+// element: 39.3e12 / 25 = 1.6e12 elements/s, which at 16 bits is 6.3 TB/s, just above the copy rate.  Measured (a copy of 1 GiB moves 5.1 TB/s):
+// 2^26 f32 0.086 ms = 6.2 TB/s, with a residual 0.125 = 6.4; 2^27 bf16 0.092 = 5.9, with a residual 0.134 = 6.0; 64000 f32 3.1 us.
 #include "lowp.h"
 
 namespace
@@ -49,7 +50,7 @@ struct DropoutArgs
 // A thread takes DROP_GRANULES 16-byte granules, a workgroup's span apart.
 constexpr int DROP_THREADS = 256, DROP_GRANULES = 4;
 
-template <int DT, bool RES>
+template <int DT, bool RES, bool STREAM>
 __global__ __launch_bounds__(DROP_THREADS) void dropout_kernel(const typename LowpType<DT>::T *__restrict__ x,
                                                                const typename LowpType<DT>::T *__restrict__ residual,
                                                                typename LowpType<DT>::T *__restrict__ y, int64_t n, DropoutArgs d,
@@ -68,9 +69,9 @@ __global__ __launch_bounds__(DROP_THREADS) void dropout_kernel(const typename Lo
     for (int i = 0; i < DROP_GRANULES; i++)
     {
         const int64_t c = (base + i * DROP_THREADS) * G;
-        L::load(x, c, n, 0.0f, v[i]);
+        L::template load<STREAM>(x, c, n, 0.0f, v[i]);
         if (RES)
-            L::load(residual, c, n, 0.0f, r[i]);
+            L::template load<STREAM>(residual, c, n, 0.0f, r[i]);
     }
 #pragma unroll
     for (int i = 0; i < DROP_GRANULES; i++)
@@ -93,7 +94,7 @@ __global__ __launch_bounds__(DROP_THREADS) void dropout_kernel(const typename Lo
                     v[i][4 * q + k] = keep ? t : 0.0f;
             }
         }
-        L::store(y, c, n, v[i]);
+        L::template store<STREAM>(y, c, n, v[i]);
     }
 }
 
@@ -104,20 +105,28 @@ __global__ void dropout_next_call_kernel(int64_t *state, int64_t *used)
     state[1] = (int64_t)((uint64_t)state[1] + 1);
 }
 
-template <int DT>
+template <int DT, bool RES, bool STREAM>
 int launch_dropout(const void *x, const void *residual, void *y, int64_t n, DropoutArgs d, const int64_t *state, uint64_t seed,
                    uint64_t call, hipStream_t s)
 {
     typedef typename LowpType<DT>::T T;
     const int64_t blocks = repdl_cdiv(n, (int64_t)Lowp<DT>::G * DROP_THREADS * DROP_GRANULES);
     REPDL_REQUIRE(blocks <= REPDL_I32_MAX);
-    if (residual != nullptr)
-        REPDL_LAUNCH((dropout_kernel<DT, true>), dim3((unsigned)blocks), dim3(DROP_THREADS), 0, s, static_cast<const T *>(x),
-                     static_cast<const T *>(residual), static_cast<T *>(y), n, d, state, seed, call);
-    else
-        REPDL_LAUNCH((dropout_kernel<DT, false>), dim3((unsigned)blocks), dim3(DROP_THREADS), 0, s, static_cast<const T *>(x),
-                     static_cast<const T *>(nullptr), static_cast<T *>(y), n, d, state, seed, call);
+    REPDL_LAUNCH((dropout_kernel<DT, RES, STREAM>), dim3((unsigned)blocks), dim3(DROP_THREADS), 0, s, static_cast<const T *>(x),
+                 static_cast<const T *>(residual), static_cast<T *>(y), n, d, state, seed, call);
     return repdl_launch_status();
+}
+
+template <int DT>
+int dropout_typed(const void *x, const void *residual, void *y, int64_t n, DropoutArgs d, const int64_t *state, uint64_t seed,
+                  uint64_t call, hipStream_t s)
+{
+    const bool stream = n >= REPDL_STREAM_BYTES / repdl_dtype_bytes(DT) && (reinterpret_cast<uintptr_t>(y) & 15) == 0;
+    if (residual != nullptr)
+        return stream ? launch_dropout<DT, true, true>(x, residual, y, n, d, state, seed, call, s)
+                      : launch_dropout<DT, true, false>(x, residual, y, n, d, state, seed, call, s);
+    return stream ? launch_dropout<DT, false, true>(x, residual, y, n, d, state, seed, call, s)
+                  : launch_dropout<DT, false, false>(x, residual, y, n, d, state, seed, call, s);
 }
 } // namespace
 
@@ -134,9 +143,9 @@ REPDL_API int repdl_hip_dropout(const void *x, const void *residual, void *y, in
     d.threshold = d.all ? 0u : (uint32_t)t;
     d.scale = d.all ? 0.0f : (float)(1.0 / (1.0 - p));
     hipStream_t s = repdl_stream(stream);
-    return dtype == REPDL_F32    ? launch_dropout<REPDL_F32>(x, residual, y, n, d, state, seed, call, s)
-           : dtype == REPDL_BF16 ? launch_dropout<REPDL_BF16>(x, residual, y, n, d, state, seed, call, s)
-                                 : launch_dropout<REPDL_F16>(x, residual, y, n, d, state, seed, call, s);
+    return dtype == REPDL_F32    ? dropout_typed<REPDL_F32>(x, residual, y, n, d, state, seed, call, s)
+           : dtype == REPDL_BF16 ? dropout_typed<REPDL_BF16>(x, residual, y, n, d, state, seed, call, s)
+                                 : dropout_typed<REPDL_F16>(x, residual, y, n, d, state, seed, call, s);
 }
 
 REPDL_API int repdl_hip_dropout_next_call(int64_t *state, int64_t *used, void *stream)

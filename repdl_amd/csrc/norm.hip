@@ -16,8 +16,8 @@
 //
 // The two passes over a row (mean, then centred squares) read it from registers: one thread holds E = 16 of its elements, as
 // 16-byte granules TPR granules apart, TPR threads a row.  Bound: HBM, 2 passes over the tensor forward and 3 backward.  Measured
-// (a copy of 1 GiB moves 5.1 TB/s): forward 16384 x 8192 bf16 0.096 ms = 5.6 TB/s, 8192 x 1024 f32 0.0130 = 5.2, 65536 x 256 f32
-// 0.027 = 5.0; backward with both launches 0.165 ms = 4.9 TB/s, 0.026 = 3.8, 0.048 = 4.2.
+// (a copy of 1 GiB moves 5.1 TB/s): forward 16384 x 8192 bf16 0.094 ms = 5.7 TB/s, 8192 x 1024 f32 0.0130 = 5.2, 65536 x 256 f32
+// 0.027 = 5.0; backward with both launches 0.166 ms = 4.8 TB/s, 0.026 = 3.8, 0.048 = 4.2.
 #include "lowp.h"
 #include "crmath.h"
 #include "lanes.h"
@@ -142,10 +142,11 @@ struct RowGranules
         }
     }
     __device__ __forceinline__ bool stores(int i) const { return skip[i] < G; }
+    template <bool STREAM>
     __device__ __forceinline__ typename L::Raw load(const typename L::T *row, int i, int N) const
     {
         if (!TINY)
-            return L::load_raw(row + at[i]);
+            return L::template load_raw<STREAM>(row + at[i]);
         typename L::Raw r = {0u, 0u, 0u, 0u};
         typename L::T t[G];
         __builtin_memcpy(t, &r, 16);
@@ -156,13 +157,11 @@ struct RowGranules
         __builtin_memcpy(&r, t, 16);
         return r;
     }
+    template <bool STREAM>
     __device__ __forceinline__ void store(typename L::T *row, int i, int N, const float *v) const
     {
         if (!TINY)
-        {
-            const typename L::Raw r = L::pack(v);
-            __builtin_memcpy(row + at[i], &r, 16);
-        }
+            L::template store_raw<STREAM>(row + at[i], L::pack(v));
         else
         {
 #pragma unroll
@@ -202,7 +201,7 @@ struct RowGranules
     }
 };
 
-template <int DT, int PDT, int TPR, int E, bool TINY>
+template <int DT, int PDT, int TPR, int E, bool TINY, bool STREAM>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_kernel(
     const typename LowpType<DT>::T *__restrict__ x, const typename LowpType<PDT>::T *__restrict__ w,
     const typename LowpType<PDT>::T *__restrict__ b, typename LowpType<DT>::T *__restrict__ y, float *__restrict__ mean_out,
@@ -221,7 +220,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_kernel(
     typename L::Raw raw[GPT];
 #pragma unroll
     for (int i = 0; i < GPT; i++)
-        raw[i] = rg.load(xr, i, N);
+        raw[i] = rg.template load<STREAM>(xr, i, N);
     float v[GPT][G];
     float s[1] = {0.0f};
 #pragma unroll
@@ -278,7 +277,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_kernel(
                 for (int k = 0; k < G; k++)
                     v[i][k] = v[i][k] + p[k];
             }
-            rg.store(yr, i, N, v[i]);
+            rg.template store<STREAM>(yr, i, N, v[i]);
         }
     }
 }
@@ -352,7 +351,7 @@ __global__ __launch_bounds__(1024) void layer_norm_long_kernel(
 // bounds a small call is a row's latency of about a microsecond and the second launch, what bounds a large one is HBM).  A
 // workgroup's 8 waves of up to 256 registers are all that its share of a CU holds: with registers for twice the waves the loop
 // spilled and ran 10-40 % slower (8192 x 4096 bf16 0.0537 -> 0.0503 ms, 100000 x 64 0.0205 -> 0.0148).
-template <int DT, int PDT, int TPR, int E, bool TINY>
+template <int DT, int PDT, int TPR, int E, bool TINY, bool STREAM>
 __global__ __launch_bounds__(ln_grad_threads(TPR), TPR < 1024 ? 2 : 4) void layer_norm_grad_kernel(
     const typename LowpType<DT>::T *__restrict__ gy, const typename LowpType<DT>::T *__restrict__ x,
     const typename LowpType<PDT>::T *__restrict__ w, const float *__restrict__ mean_in, const float *__restrict__ rstd_in,
@@ -391,8 +390,8 @@ __global__ __launch_bounds__(ln_grad_threads(TPR), TPR < 1024 ? 2 : 4) void laye
 #pragma unroll
         for (int i = 0; i < GPT; i++)
         {
-            nx[i] = rg.load(x + rr * N, i, N);
-            ng[i] = rg.load(gy + rr * N, i, N);
+            nx[i] = rg.template load<STREAM>(x + rr * N, i, N);
+            ng[i] = rg.template load<STREAM>(gy + rr * N, i, N);
         }
         next_mean = mean_in[rr];
         next_rstd = rstd_in[rr];
@@ -469,7 +468,7 @@ __global__ __launch_bounds__(ln_grad_threads(TPR), TPR < 1024 ? 2 : 4) void laye
 #pragma unroll
                     for (int k = 0; k < G; k++)
                         o[k] = rstd * ((gv[i][k] - m1) - xv[i][k] * m2);
-                    rg.store(gx + row * N, i, N, o);
+                    rg.template store<STREAM>(gx + row * N, i, N, o);
                 }
             }
         }
@@ -641,6 +640,14 @@ __global__ __launch_bounds__(64 * LN_FOLD) void layer_norm_param_kernel(const fl
 }
 
 // ---- host -------------------------------------------------------------------------------------
+// Large tensors go past the caches (4096 x 16384 f32 forward 0.103 -> 0.096 ms, backward 0.181 -> 0.162): rows that a wave or more
+// shares, on 16-byte boundaries.
+template <int DT>
+bool ln_streams(int64_t M, int64_t N, const void *out)
+{
+    return M * N >= REPDL_STREAM_BYTES / repdl_dtype_bytes(DT) && N % Lowp<DT>::G == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+}
+
 template <int DT, int PDT, int TPR, bool TINY = false>
 int launch_layer_norm(const void *x, const void *w, const void *b, void *y, float *mean, float *rstd, int64_t M, int64_t N, float eps,
                       hipStream_t s)
@@ -648,9 +655,15 @@ int launch_layer_norm(const void *x, const void *w, const void *b, void *y, floa
     typedef typename LowpType<DT>::T T;
     typedef typename LowpType<PDT>::T P;
     constexpr int THREADS = TPR < 256 ? 256 : TPR, TEAMS = THREADS / TPR;
-    REPDL_LAUNCH((layer_norm_kernel<DT, PDT, TPR, LN_E, TINY>), dim3((unsigned)repdl_cdiv(M, TEAMS)), dim3(THREADS), 0, s,
-                 static_cast<const T *>(x), static_cast<const P *>(w), static_cast<const P *>(b), static_cast<T *>(y), mean, rstd, M, (int)N,
-                 (float)(1.0 / (double)N), eps);
+    const dim3 grid((unsigned)repdl_cdiv(M, TEAMS));
+    if (TPR >= 64 && ln_streams<DT>(M, N, y))
+        REPDL_LAUNCH((layer_norm_kernel<DT, PDT, TPR, LN_E, TINY, (TPR >= 64)>), grid, dim3(THREADS), 0, s, static_cast<const T *>(x),
+                     static_cast<const P *>(w), static_cast<const P *>(b), static_cast<T *>(y), mean, rstd, M, (int)N,
+                     (float)(1.0 / (double)N), eps);
+    else
+        REPDL_LAUNCH((layer_norm_kernel<DT, PDT, TPR, LN_E, TINY, false>), grid, dim3(THREADS), 0, s, static_cast<const T *>(x),
+                     static_cast<const P *>(w), static_cast<const P *>(b), static_cast<T *>(y), mean, rstd, M, (int)N,
+                     (float)(1.0 / (double)N), eps);
     return repdl_launch_status();
 }
 
@@ -700,9 +713,15 @@ int launch_layer_norm_grad(const void *gy, const void *x, const void *w, const f
     typedef typename LowpType<DT>::T T;
     typedef typename LowpType<PDT>::T P;
     const int64_t rpb = ln_rows_per_block(M, N);
-    REPDL_LAUNCH((layer_norm_grad_kernel<DT, PDT, TPR, LN_E, TINY>), dim3((unsigned)repdl_cdiv(M, rpb)), dim3(ln_grad_threads(TPR)), 0, s,
-                 static_cast<const T *>(gy), static_cast<const T *>(x), static_cast<const P *>(w), mean, rstd, static_cast<T *>(gx), partial,
-                 M, (int)N, rpb, (float)(1.0 / (double)N));
+    const dim3 grid((unsigned)repdl_cdiv(M, rpb)), block(ln_grad_threads(TPR));
+    if (TPR >= 64 && ln_streams<DT>(M, N, gx))
+        REPDL_LAUNCH((layer_norm_grad_kernel<DT, PDT, TPR, LN_E, TINY, (TPR >= 64)>), grid, block, 0, s, static_cast<const T *>(gy),
+                     static_cast<const T *>(x), static_cast<const P *>(w), mean, rstd, static_cast<T *>(gx), partial, M, (int)N, rpb,
+                     (float)(1.0 / (double)N));
+    else
+        REPDL_LAUNCH((layer_norm_grad_kernel<DT, PDT, TPR, LN_E, TINY, false>), grid, block, 0, s, static_cast<const T *>(gy),
+                     static_cast<const T *>(x), static_cast<const P *>(w), mean, rstd, static_cast<T *>(gx), partial, M, (int)N, rpb,
+                     (float)(1.0 / (double)N));
     return repdl_launch_status();
 }
 

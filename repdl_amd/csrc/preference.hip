@@ -15,9 +15,9 @@
 //
 // Bound: HBM, and for 16-bit logits level with it the vector ALU.  A column of the forward pass is 13 instructions -- widen, half
 // a maximum, clamp, 9 of crm_exp_term, an addition -- so 39.3e12 / 13 = 3e12 columns/s are 6 TB/s of 16-bit ones.  Measured, three
-// quarters of the tokens counted: 8192 x 131072 bf16 forward 0.295 ms = 5.45 TB/s read (0.351 with the exponential as
-// crm_exp_neg of a difference, 16 instructions; 0.275 with the hardware's exponential, whose bits are its own), backward 0.657 ms =
-// 5.7 TB/s; 8192 x 32000 f32 forward 0.135 ms = 5.8, backward 0.344 = 5.3; a pair of 12 tokens x 1000 7 + 5 us.
+// quarters of the tokens counted: 8192 x 131072 bf16 forward 0.281 ms = 5.7 TB/s read (0.351 with the exponential as
+// crm_exp_neg of a difference, 16 instructions; degree 6 here 0.304), backward 0.660 ms = 5.7 TB/s; 8192 x 32000 f32 forward 0.120 ms =
+// 6.5, backward 0.340 = 5.4; a pair of 12 tokens x 1000 7 + 5 us.
 //
 // The row sum is in binary32 in a fixed order (a thread's granules in turn, a butterfly over the wave, the waves, the chunks),
 // which the vocabulary and the type determine alone.  Everything per token and per pair after it is in binary64: L is a sum
@@ -51,7 +51,7 @@ __device__ __forceinline__ const T *pref_row(const T *x, const PrefShape &p, uin
 }
 
 // TPR threads share the E * TPR columns (at most) of one chunk of a row: 64 where a wave holds the whole row, else a workgroup.
-template <int DT, int TPR, int E>
+template <int DT, int TPR, int E, bool STREAM>
 __global__ __launch_bounds__(256) void preference_rows_kernel(const typename LowpType<DT>::T *__restrict__ x,
                                                               const int64_t *__restrict__ target, float2 *__restrict__ part,
                                                               float *__restrict__ picked, int *__restrict__ counter, PrefShape p)
@@ -85,7 +85,7 @@ __global__ __launch_bounds__(256) void preference_rows_kernel(const typename Low
     {
         const int c = (i * TPR + j) * G;
         if (c + G <= width)
-            raw[i] = L::load_raw(xr + c0 + c);
+            raw[i] = L::template load_raw<STREAM>(xr + c0 + c);
     }
     float m = none;
 #pragma unroll
@@ -313,7 +313,7 @@ __global__ __launch_bounds__(PAIR_THREADS) void preference_pairs_kernel(const in
 }
 
 // d loss / d x: k e^(x - m) with k = -c / sum, and c more at the target.
-template <int DT, int TPR, int E>
+template <int DT, int TPR, int E, bool STREAM>
 __global__ __launch_bounds__(256, 4) void preference_grad_kernel(const typename LowpType<DT>::T *__restrict__ x,
                                                               const int64_t *__restrict__ target,
                                                               const float2 *__restrict__ row_stats, const float *__restrict__ coef,
@@ -344,7 +344,7 @@ __global__ __launch_bounds__(256, 4) void preference_grad_kernel(const typename 
         {
             const int c = (i * TPR + j) * G;
             if (c < width)
-                L::store(gr, c, width, v);
+                L::template store<STREAM>(gr, c, width, v);
         }
         return;
     }
@@ -355,7 +355,7 @@ __global__ __launch_bounds__(256, 4) void preference_grad_kernel(const typename 
     {
         const int c = (i * TPR + j) * G;
         if (c + G <= width)
-            raw[i] = L::load_raw(xr + c);
+            raw[i] = L::template load_raw<STREAM>(xr + c);
     }
     const float2 st = row_stats[row];
     const float cc = coef[row / (uint32_t)p.steps] * *grad_loss;
@@ -384,7 +384,7 @@ __global__ __launch_bounds__(256, 4) void preference_grad_kernel(const typename 
                 for (int k = 0; k < G; k++)
                     v[k] = at == c + k ? v[k] + cc : v[k];
             }
-            L::store(gr, c, width, v);
+            L::template store<STREAM>(gr, c, width, v);
         }
     }
 }
@@ -427,6 +427,12 @@ PrefShape pref_shape(int64_t pairs, int64_t steps, int64_t vocab, int64_t seq_st
 }
 
 template <int DT>
+bool pref_streams(const PrefShape &p)
+{
+    return (int64_t)p.rows * p.vocab >= REPDL_STREAM_BYTES / repdl_dtype_bytes(DT);
+}
+
+template <int DT>
 int launch_pref_rows(const void *logits, const int64_t *target, float2 *part, float *picked, int *counter, const PrefShape &p, hipStream_t s)
 {
     const auto *x = static_cast<const typename LowpType<DT>::T *>(logits);
@@ -434,11 +440,13 @@ int launch_pref_rows(const void *logits, const int64_t *target, float2 *part, fl
     const unsigned by_wave = (unsigned)(p.rows == 0 ? 1 : repdl_cdiv(p.rows, 4));
     const unsigned by_chunk = (unsigned)(p.rows == 0 ? 1 : (int64_t)p.rows * p.chunks);
     if (p.vocab <= PREF_WAVE_SMALL)
-        REPDL_LAUNCH((preference_rows_kernel<DT, 64, PREF_SMALL_E>), dim3(by_wave), dim3(256), 0, s, x, target, part, picked, counter, p);
+        REPDL_LAUNCH((preference_rows_kernel<DT, 64, PREF_SMALL_E, false>), dim3(by_wave), dim3(256), 0, s, x, target, part, picked, counter, p);
     else if (p.vocab <= PREF_WAVE)
-        REPDL_LAUNCH((preference_rows_kernel<DT, 64, PREF_E>), dim3(by_wave), dim3(256), 0, s, x, target, part, picked, counter, p);
+        REPDL_LAUNCH((preference_rows_kernel<DT, 64, PREF_E, false>), dim3(by_wave), dim3(256), 0, s, x, target, part, picked, counter, p);
+    else if (pref_streams<DT>(p))
+        REPDL_LAUNCH((preference_rows_kernel<DT, 256, PREF_E, true>), dim3(by_chunk), dim3(256), 0, s, x, target, part, picked, counter, p);
     else
-        REPDL_LAUNCH((preference_rows_kernel<DT, 256, PREF_E>), dim3(by_chunk), dim3(256), 0, s, x, target, part, picked, counter, p);
+        REPDL_LAUNCH((preference_rows_kernel<DT, 256, PREF_E, false>), dim3(by_chunk), dim3(256), 0, s, x, target, part, picked, counter, p);
     return repdl_launch_status();
 }
 
@@ -452,10 +460,13 @@ int launch_pref_grad(const void *logits, const int64_t *target, const float2 *ro
     const T *x = static_cast<const T *>(logits);
     T *gx = static_cast<T *>(grad_logits);
     if (p.vocab <= PREF_WAVE_SMALL)
-        REPDL_LAUNCH((preference_grad_kernel<DT, 64, PREF_SMALL_E>), dim3((unsigned)repdl_cdiv(p.rows, 4)), dim3(256), 0, s, x, target,
+        REPDL_LAUNCH((preference_grad_kernel<DT, 64, PREF_SMALL_E, false>), dim3((unsigned)repdl_cdiv(p.rows, 4)), dim3(256), 0, s, x, target,
                      row_stats, coef, grad_loss, gx, p);
+    else if (pref_streams<DT>(p) && p.vocab % Lowp<DT>::G == 0 && (reinterpret_cast<uintptr_t>(gx) & 15) == 0)
+        REPDL_LAUNCH((preference_grad_kernel<DT, 256, PREF_GRAD_E, true>), dim3((unsigned)((int64_t)p.rows * p.chunks)), dim3(256), 0, s, x,
+                     target, row_stats, coef, grad_loss, gx, p);
     else
-        REPDL_LAUNCH((preference_grad_kernel<DT, 256, PREF_GRAD_E>), dim3((unsigned)((int64_t)p.rows * p.chunks)), dim3(256), 0, s, x,
+        REPDL_LAUNCH((preference_grad_kernel<DT, 256, PREF_GRAD_E, false>), dim3((unsigned)((int64_t)p.rows * p.chunks)), dim3(256), 0, s, x,
                      target, row_stats, coef, grad_loss, gx, p);
     return repdl_launch_status();
 }

@@ -12,9 +12,9 @@ pytestmark = pytest.mark.gpu
 TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
 
 
-def expected(x, p, seed, call, residual=None):
+def expected(x, p, seed, call, residual=None, first=0):
     """The definition with its roundings: one product in binary32, one sum in binary32, one rounding to the type."""
-    keep = torch.from_numpy(philox.words(x.numel(), seed, call).astype(np.int64)).view(x.shape) >= round(p * 2 ** 32)
+    keep = torch.from_numpy(philox.words(x.numel(), seed, call, first).astype(np.int64)).view(x.shape) >= round(p * 2 ** 32)
     scaled = x.float() * torch.tensor(1 / (1 - p), dtype=torch.float32) if p < 1 else torch.zeros_like(x.float())
     if residual is None:
         return torch.where(keep, scaled, torch.zeros(())).to(x.dtype), keep
@@ -182,6 +182,23 @@ def test_side_stream_and_both_bindings():
     state = torch.tensor([1, 1], device="cuda")
     assert torch.equal(hip_ctypes.dropout(x, x, 0.3, state, 0, 0), want)
     assert hip_ctypes.dropout_next_call(state).tolist() == [1, 1] and state.tolist() == [1, 2]
+
+
+@pytest.mark.parametrize("kind", sorted(TYPES))
+@pytest.mark.parametrize("residual", [False, True])
+def test_large_tensors_have_the_bits_of_their_beginning(kind, residual):
+    """256 MB and more are moved past the caches, by other instructions."""
+    from repdl_amd import ops
+
+    n = (1 << 28) // torch.finfo(TYPES[kind]).bits * 8 + 77
+    x = gen.normal_like(80, 1 << 20).to(TYPES[kind]).cuda().repeat((n >> 20) + 1)[:n]
+    r = x.flip(0) if residual else None
+    y = ops.dropout(x, 0.3, (8, 9), r)
+    m = n // 2 + 3
+    assert torch.equal(y[:m], ops.dropout(x[:m], 0.3, (8, 9), r[:m] if residual else None))
+    first = (n - 4096) // 4 * 4  # and the end against the definition
+    want, _ = expected(x[first:].cpu(), 0.3, 8, 9, r[first:].cpu() if residual else None, first)
+    assert torch.equal(y[first:].cpu(), want)
 
 
 def test_more_elements_than_32_bits_count():

@@ -266,6 +266,25 @@ def test_bits_of_the_documented_order(shape, kind):
         assert torch.equal(got.cpu(), torch.from_numpy(want).to(got.dtype))
 
 
+@pytest.mark.parametrize("kind", sorted(TYPES))
+@pytest.mark.parametrize("cols", [1000, 2048, 4096, 8192, 16384])
+def test_large_tensors_have_the_bits_of_their_parts(kind, cols):
+    """256 MB and more are moved past the caches, by other instructions."""
+    from repdl_amd import ops
+
+    t = TYPES[kind]
+    rows = (1 << 28) // torch.finfo(t).bits * 8 // cols + 5
+    x = gen.normal_like(123, 257, cols).to(t).cuda().repeat(rows // 257 + 1, 1)[:rows]
+    w, b = gen.normal_like(124, cols).to(t).cuda(), gen.normal_like(125, cols).to(t).cuda()
+    gy = x.flip(0)
+    y, mean, rstd = ops.layer_norm(x, (cols,), w, b)
+    gx = ops.layer_norm_grad(gy, x, mean, rstd, (cols,), w)[0]
+    for at in (slice(0, 300), slice(rows - 300, rows)):
+        want = ops.layer_norm(x[at], (cols,), w, b)
+        assert torch.equal(y[at], want[0]) and torch.equal(mean[at], want[1]) and torch.equal(rstd[at], want[2])
+        assert torch.equal(gx[at], ops.layer_norm_grad(gy[at], x[at], want[1], want[2], (cols,), w)[0])
+
+
 def test_more_elements_than_32_bits_count():
     from repdl_amd import ops
 

@@ -264,10 +264,32 @@ def test_many_pairs_in_order():
         assert torch.equal(again[0], loss) and torch.equal(again[1], logps)
 
 
-def test_more_elements_than_32_bits_count():
+@pytest.mark.parametrize("kind", sorted(TYPES))
+@pytest.mark.parametrize("vocab", [6000, 20480])
+def test_large_tensors_have_the_bits_of_their_parts(vocab, kind):
+    """256 MB and more are moved past the caches, by other instructions: two pairs against each alone, whose gradient is twice as large."""
     from repdl_amd import ops
 
-    P, S, V = 2, 8200, 65536 + 3                      # 2.15e9 elements
+    t = TYPES[kind]
+    S = (1 << 28) // torch.finfo(t).bits * 8 // (4 * vocab) + 1
+    x = gen.normal_like(90, 4, 64, vocab).mul(2).to(t).cuda().repeat(1, S // 64 + 1, 1)[:, :S].contiguous()
+    target = gen.labels(91, 4 * S, vocab).view(4, S).cuda()
+    target[:, S // 2:S // 2 + 9] = -100
+    one = torch.ones((), device="cuda")
+    loss, logps, stats, coef = ops.preference_loss(x, target, None, 1e-3)
+    g = ops.preference_loss_grad(x, target, stats, coef, one)
+    for pair in ([0, 2], [1, 3]):
+        px, pt = x[pair], target[pair]
+        _, plogps, pstats, pcoef = ops.preference_loss(px, pt, None, 1e-3)
+        assert torch.equal(plogps, logps[pair]) and torch.equal(pcoef, 2 * coef[pair])
+        assert torch.equal(ops.preference_loss_grad(px, pt, pstats, pcoef, one * 0.5), g[pair])
+
+
+@pytest.mark.parametrize("V", [65536, 65536 + 3])
+def test_more_elements_than_32_bits_count(V):
+    from repdl_amd import ops
+
+    P, S = 2, 8200                                    # 2.15e9 elements
     x = torch.zeros(2 * P, S, V, dtype=torch.bfloat16, device="cuda")
     tail = gen.normal_like(86, 8, V).to(torch.bfloat16).cuda()
     x[-1, -8:] = tail
