@@ -17,9 +17,9 @@ and ``cross_entropy``.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 
@@ -484,6 +484,33 @@ def preference_loss_grad(logits, target, row_stats, coef, grad_loss, ignore_inde
 # ---- autograd: the differentiable forms, as csrc/bind.cpp has them ----
 
 
+class _Once(torch.autograd.Function):
+    """The gradients as they are; differentiating them again is an error."""
+
+    @staticmethod
+    def forward(ctx, *grads):
+        return tuple(None if g is None else g.view_as(g) for g in grads)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("this function can be differentiated only once")
+
+
+def _once(backward):
+    """Backward functions whose gradients are not differentiable: where the backward pass is recorded, differentiating them
+    again is an error, not a silent zero."""
+
+    @functools.wraps(backward)
+    def wrapped(ctx, *grads):
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return out
+        return _Once.apply(*(None if g is None else g.detach().requires_grad_() for g in out))
+
+    return wrapped
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, n, weight, bias, eps):
@@ -493,7 +520,7 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, gy):
         x, weight, bias, mean, rstd = ctx.saved_tensors
         need_x, _, need_w, need_b = ctx.needs_input_grad[:4]
@@ -513,7 +540,7 @@ class _Dropout(torch.autograd.Function):
         return dropout(x, residual, p, state, seed, call)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, gy):
         p, seed, call = ctx.rest
         # the mask again, from the same call of the generator
@@ -536,7 +563,7 @@ class _Preference(torch.autograd.Function):
         return loss, logps
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g, _):
         if g is None:
             return (None,) * 6

@@ -579,13 +579,11 @@ namespace
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-// Gradients of a function that is differentiable once: differentiating them again is an error, not a silent zero.
-variable_list once(variable_list grads, const variable_list &incoming)
+// Gradients of a function that is differentiable once: where the backward pass is recorded, differentiating them again is an
+// error, not a silent zero.
+variable_list once(variable_list grads)
 {
-    bool recorded = false;
-    for (const auto &g : incoming)
-        recorded = recorded || (g.defined() && g.requires_grad());
-    if (!at::GradMode::is_enabled() || !recorded)
+    if (!at::GradMode::is_enabled())
         return grads;
     for (auto &g : grads)
         if (g.defined())
@@ -627,7 +625,7 @@ struct LayerNormFunction : public torch::autograd::Function<LayerNormFunction>
             gw = gw.view(ctx->saved_data["shape"].toIntVector());
         if (gb.defined())
             gb = gb.view(ctx->saved_data["shape"].toIntVector());
-        return once({std::get<0>(r), gw, gb, torch::Tensor(), torch::Tensor()}, grads);
+        return once({std::get<0>(r), gw, gb, torch::Tensor(), torch::Tensor()});
     }
 };
 
@@ -656,7 +654,7 @@ struct DropoutFunction : public torch::autograd::Function<DropoutFunction>
                          (uint64_t)ctx->saved_data["call"].toInt());
         if (ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(1))
             gr = grads[0];
-        return once({gx, gr, torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor()}, grads);
+        return once({gx, gr, torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor()});
     }
 };
 
@@ -680,7 +678,7 @@ struct PreferenceFunction : public torch::autograd::Function<PreferenceFunction>
             const auto saved = ctx->get_saved_variables();
             g = preference_loss_grad(saved[0], saved[1], saved[2], saved[3], grads[0], ctx->saved_data["ignore"].toInt());
         }
-        return once({g, torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor()}, grads);
+        return once({g, torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor()});
     }
 };
 } // namespace

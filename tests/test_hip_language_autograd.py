@@ -76,13 +76,14 @@ def test_a_second_derivative_is_refused(binding):
     x, w, b, t = _inputs()
     x.requires_grad_()
     outs = [lambda: F.layer_norm(x, 40, w, b).square().sum(), lambda: F.dropout(x, 0.5, (1, 2)).square().sum(),
-            lambda: F.preference_loss(x.view(2, 3, 40), t)[0].square()]
+            lambda: F.preference_loss(x.view(2, 3, 40), t)[0].square(),
+            lambda: F.preference_loss(x.view(2, 3, 40), t)[0], lambda: F.layer_norm(x, 40, w, b).sum(), lambda: F.dropout(x, 0.5, (1, 2)).sum()]
     for f in outs:
         (g,) = torch.autograd.grad(f(), x)
         (h,) = torch.autograd.grad(f(), x, create_graph=True)  # (the first derivative of a recorded backward pass is there)
-        assert torch.equal(g, h.detach())
-        with pytest.raises(RuntimeError):
-            h.sum().backward()
+        assert torch.equal(g, h.detach()) and h.requires_grad
+        with pytest.raises(RuntimeError, match="only once"):
+            (x.sum() + h.square().sum()).backward()  # (a penalty on the gradient, beside a term that has one)
 
 
 def test_a_changed_input_is_noticed(binding):
