@@ -314,7 +314,8 @@ int repdl_hip_bn_gweight_term(const float *x, const float *mean, const float *st
  *   grad_weight = S over the rows of RN(grad_y_ij * xh_ij),  grad_bias = S over the rows of grad_y_ij
  * (the order of the sums over rows is a function of M, N and the type; they are rounded to param_dtype at the end).  Any of
  * grad_x, grad_weight, grad_bias may be NULL: not wanted.  M = 0 gives zeros in grad_weight and grad_bias.
- * Scratch (see "Scratch memory"): at most 512 rows of 2 N floats for the two sums over rows. */
+ * Scratch (see "Scratch memory"): at most 512 rows of 2 N floats for the two sums over rows, where they are wanted; none for at
+ * most 256 rows of at most 16384 elements. */
 int repdl_hip_layer_norm(const void *x, const void *weight, const void *bias, void *y, float *mean, float *rstd, int64_t M,
                          int64_t N, float eps, int dtype, int param_dtype, void *stream);
 int repdl_hip_layer_norm_grad(const void *grad_y, const void *x, const void *weight, const float *mean, const float *rstd,

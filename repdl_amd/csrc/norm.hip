@@ -12,7 +12,7 @@
 //   over a row   a granule's elements in pairs, pairs of pairs, ...; a thread's granules in turn; the threads of a wave as a
 //                butterfly; the waves in turn;
 //   over rows    a workgroup's run of rows, each of its teams taking every (number of teams)-th one in turn; the teams in turn; sixteen
-//                sums of every sixteenth run; those in turn.
+//                sums of every sixteenth run; those in turn.  At most 256 rows: 16 to 64 sums of every 16th to 64th row, those in turn.
 //
 // The two passes over a row (mean, then centred squares) read it from registers: one thread holds E = 16 of its elements, as
 // 16-byte granules TPR granules apart, TPR threads a row.  Bound: HBM, 2 passes over the tensor forward and 3 backward.  Measured
@@ -516,6 +516,156 @@ __global__ __launch_bounds__(ln_grad_threads(TPR), TPR < 1024 ? 2 : 4) void laye
     }
 }
 
+// Few rows: one launch for all three gradients.  The first `row_blocks` workgroups make gx, a row per team; the others make gw and gb
+// straight from x, gy and the rows' statistics, 16 granules of columns a workgroup, every 16 threads taking every
+// (threads / 16)-th row in turn and their sums added in order through LDS.  x and gy are read twice, the second time out of
+// the caches, and there are no partial sums, no second launch and no scratch.
+template <int DT, int PDT, int TPR, int E, bool TINY>
+__global__ __launch_bounds__(ln_grad_threads(TPR)) void layer_norm_grad_few_kernel(
+    const typename LowpType<DT>::T *__restrict__ gy, const typename LowpType<DT>::T *__restrict__ x,
+    const typename LowpType<PDT>::T *__restrict__ w, const float *__restrict__ mean_in, const float *__restrict__ rstd_in,
+    typename LowpType<DT>::T *__restrict__ gx, typename LowpType<PDT>::T *__restrict__ gw, typename LowpType<PDT>::T *__restrict__ gb,
+    int M, int N, int row_blocks, float inv_n)
+{
+    typedef Lowp<DT> L;
+    constexpr int G = L::G, GPT = E / G;
+    constexpr int THREADS = ln_grad_threads(TPR), TEAMS = THREADS / TPR, GROUPS = THREADS / 16;
+    __shared__ float scratch[TEAMS][2 * (TPR / 64) + 1];
+    __shared__ float fold[GROUPS][16 * G];
+    const int tid = threadIdx.x;
+    if ((int)blockIdx.x < row_blocks)
+    {
+        const int team = tid / TPR, j = tid % TPR;
+        const int64_t row = wave_value<TPR>((int64_t)blockIdx.x * TEAMS + team);
+        const bool live = row < M;
+        const int64_t rr = live ? row : M - 1;
+        const RowGranules<DT, TPR, E, TINY> rg(N, j);
+        typename L::Raw rx[GPT], rgy[GPT];
+#pragma unroll
+        for (int i = 0; i < GPT; i++)
+        {
+            rx[i] = rg.template load<false>(x + rr * N, i, N);
+            rgy[i] = rg.template load<false>(gy + rr * N, i, N);
+        }
+        const float mean = mean_in[rr], rstd = rstd_in[rr];
+        float xv[GPT][G], gv[GPT][G];
+        float s[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < GPT; i++)
+        {
+            float p[G];
+            L::unpack(rx[i], xv[i]);
+            L::unpack(rgy[i], gv[i]);
+            if (w != nullptr)
+            {
+                rg.template param<PDT>(w, i, N, p);
+#pragma unroll
+                for (int k = 0; k < G; k++)
+                    gv[i][k] = gv[i][k] * p[k];
+            }
+#pragma unroll
+            for (int k = 0; k < G; k++)
+            {
+                xv[i][k] = (xv[i][k] - mean) * rstd;
+                p[k] = gv[i][k] * xv[i][k];
+            }
+            s[0] = s[0] + rg.sum(gv[i], i, N);
+            s[1] = s[1] + rg.sum(p, i, N);
+        }
+        team_sum<TPR, 2>(s, scratch[team], j);
+        const float m1 = s[0] * inv_n, m2 = s[1] * inv_n;
+        if (live)
+        {
+#pragma unroll
+            for (int i = 0; i < GPT; i++)
+                if (rg.stores(i))
+                {
+                    float o[G];
+#pragma unroll
+                    for (int k = 0; k < G; k++)
+                        o[k] = rstd * ((gv[i][k] - m1) - xv[i][k] * m2);
+                    rg.template store<false>(gx + row * N, i, N, o);
+                }
+        }
+        return;
+    }
+    // columns c .. c+G-1 (the last granule of the row starts earlier where it would cross the end, see RowGranules)
+    const int lane = tid % 16, group = tid / 16;
+    const int wanted = (((int)blockIdx.x - row_blocks) * 16 + lane) * G;
+    const int c = TINY ? 0 : (wanted < N - G ? wanted : N - G);
+    float aw[G], ab[G];
+#pragma unroll
+    for (int k = 0; k < G; k++)
+        aw[k] = ab[k] = 0.0f;
+    constexpr int AHEAD = 4; // rows under way at once
+    for (int base = group; base < M; base += AHEAD * GROUPS)
+    {
+        typename L::Raw rx[AHEAD], rgy[AHEAD];
+        float mean[AHEAD], rstd[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++)
+        {
+            const int row = base + u * GROUPS < M ? base + u * GROUPS : M - 1;
+            const int64_t at = (int64_t)row * N + c;
+            if (!TINY)
+            {
+                rx[u] = L::load_raw(x + at);
+                rgy[u] = L::load_raw(gy + at);
+            }
+            else
+            {
+                float v[G];
+                L::load(x + at, 0, N, 0.0f, v);
+                rx[u] = L::pack(v);
+                L::load(gy + at, 0, N, 0.0f, v);
+                rgy[u] = L::pack(v);
+            }
+            mean[u] = mean_in[row];
+            rstd[u] = rstd_in[row];
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++)
+        {
+            float xv[G], gv[G];
+            L::unpack(rx[u], xv);
+            L::unpack(rgy[u], gv);
+            if (base + u * GROUPS < M)
+            {
+#pragma unroll
+                for (int k = 0; k < G; k++)
+                {
+                    aw[k] = aw[k] + gv[k] * ((xv[k] - mean[u]) * rstd[u]);
+                    ab[k] = ab[k] + gv[k];
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int which = 0; which < 2; which++)
+    {
+        typename LowpType<PDT>::T *out = which == 0 ? gw : gb;
+        if (out == nullptr)
+            continue;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < G; k++)
+            fold[group][lane * G + k] = which == 0 ? aw[k] : ab[k];
+        __syncthreads();
+        if (tid < 16 * G)
+        {
+            float s = fold[0][tid];
+#pragma unroll 8
+            for (int g = 1; g < GROUPS; g++)
+                s = s + fold[g][tid];
+            // this thread's column: granule tid / G of the workgroup, whose start may have been moved
+            const int start = (((int)blockIdx.x - row_blocks) * 16 + tid / G) * G;
+            const int col = (TINY ? 0 : (start < N - G ? start : N - G)) + tid % G;
+            if (start < N && col < N)
+                out[col] = LowpType<PDT>::narrow(s);
+        }
+    }
+}
+
 // The same for rows too long for the registers: gx by a workgroup per row that reads it twice ...
 template <int DT, int PDT>
 __global__ __launch_bounds__(1024) void layer_norm_grad_long_kernel(
@@ -706,12 +856,27 @@ int64_t ln_rows_per_block(int64_t M, int64_t N)
     return repdl_cdiv(repdl_cdiv(M, tpr < 512 ? 512 : 256), teams) * teams;
 }
 
+// Rows up to which one launch makes all gradients (layer_norm_grad_few_kernel).  Both sides, two launches against one: 64 x 1024 f32
+// 0.0081 / 0.0054 ms, 256 x 1024 0.0081 / 0.0058, 256 x 8192 0.0167 / 0.0090, 256 x 4096 bf16 0.0109 / 0.0076; 512 x 1024 f32 0.0081 / 0.0089,
+// 1024 x 4096 bf16 0.0177 / 0.0244.
+constexpr int64_t LN_FEW_ROWS = 256;
+bool ln_few_rows(int64_t M, int64_t N) { return M <= LN_FEW_ROWS && N <= LN_MAX_ONCHIP; }
+
 template <int DT, int PDT, int TPR, bool TINY = false>
-int launch_layer_norm_grad(const void *gy, const void *x, const void *w, const float *mean, const float *rstd, void *gx, float *partial,
-                           int64_t M, int64_t N, hipStream_t s)
+int launch_layer_norm_grad(const void *gy, const void *x, const void *w, const float *mean, const float *rstd, void *gx, void *gw, void *gb,
+                           float *partial, int64_t M, int64_t N, hipStream_t s)
 {
     typedef typename LowpType<DT>::T T;
     typedef typename LowpType<PDT>::T P;
+    if (ln_few_rows(M, N))
+    {
+        const int rows = gx != nullptr ? (int)repdl_cdiv(M, ln_grad_threads(TPR) / TPR) : 0;
+        const int cols = gw != nullptr || gb != nullptr ? (int)repdl_cdiv(N, 16 * Lowp<DT>::G) : 0;
+        REPDL_LAUNCH((layer_norm_grad_few_kernel<DT, PDT, TPR, LN_E, TINY>), dim3((unsigned)(rows + cols)), dim3(ln_grad_threads(TPR)), 0, s,
+                     static_cast<const T *>(gy), static_cast<const T *>(x), static_cast<const P *>(w), mean, rstd, static_cast<T *>(gx),
+                     static_cast<P *>(gw), static_cast<P *>(gb), (int)M, (int)N, rows, (float)(1.0 / (double)N));
+        return repdl_launch_status();
+    }
     const int64_t rpb = ln_rows_per_block(M, N);
     const dim3 grid((unsigned)repdl_cdiv(M, rpb)), block(ln_grad_threads(TPR));
     if (TPR >= 64 && ln_streams<DT>(M, N, gx))
@@ -726,8 +891,8 @@ int launch_layer_norm_grad(const void *gy, const void *x, const void *w, const f
 }
 
 template <int DT, int PDT>
-int layer_norm_grad_typed(const void *gy, const void *x, const void *w, const float *mean, const float *rstd, void *gx, float *partial,
-                          int64_t M, int64_t N, hipStream_t s)
+int layer_norm_grad_typed(const void *gy, const void *x, const void *w, const float *mean, const float *rstd, void *gx, void *gw, void *gb,
+                          float *partial, int64_t M, int64_t N, hipStream_t s)
 {
     typedef typename LowpType<DT>::T T;
     typedef typename LowpType<PDT>::T P;
@@ -747,18 +912,18 @@ int layer_norm_grad_typed(const void *gy, const void *x, const void *w, const fl
         return repdl_launch_status();
     }
     if (N < Lowp<DT>::G)
-        return launch_layer_norm_grad<DT, PDT, 4, true>(gy, x, w, mean, rstd, gx, partial, M, N, s);
+        return launch_layer_norm_grad<DT, PDT, 4, true>(gy, x, w, mean, rstd, gx, gw, gb, partial, M, N, s);
     switch (ln_threads_per_row(N, LN_E))
     {
-    case 4: return launch_layer_norm_grad<DT, PDT, 4>(gy, x, w, mean, rstd, gx, partial, M, N, s);
-    case 8: return launch_layer_norm_grad<DT, PDT, 8>(gy, x, w, mean, rstd, gx, partial, M, N, s);
-    case 16: return launch_layer_norm_grad<DT, PDT, 16>(gy, x, w, mean, rstd, gx, partial, M, N, s);
-    case 32: return launch_layer_norm_grad<DT, PDT, 32>(gy, x, w, mean, rstd, gx, partial, M, N, s);
-    case 64: return launch_layer_norm_grad<DT, PDT, 64>(gy, x, w, mean, rstd, gx, partial, M, N, s);
-    case 128: return launch_layer_norm_grad<DT, PDT, 128>(gy, x, w, mean, rstd, gx, partial, M, N, s);
-    case 256: return launch_layer_norm_grad<DT, PDT, 256>(gy, x, w, mean, rstd, gx, partial, M, N, s);
-    case 512: return launch_layer_norm_grad<DT, PDT, 512>(gy, x, w, mean, rstd, gx, partial, M, N, s);
-    default: return launch_layer_norm_grad<DT, PDT, 1024>(gy, x, w, mean, rstd, gx, partial, M, N, s);
+    case 4: return launch_layer_norm_grad<DT, PDT, 4>(gy, x, w, mean, rstd, gx, gw, gb, partial, M, N, s);
+    case 8: return launch_layer_norm_grad<DT, PDT, 8>(gy, x, w, mean, rstd, gx, gw, gb, partial, M, N, s);
+    case 16: return launch_layer_norm_grad<DT, PDT, 16>(gy, x, w, mean, rstd, gx, gw, gb, partial, M, N, s);
+    case 32: return launch_layer_norm_grad<DT, PDT, 32>(gy, x, w, mean, rstd, gx, gw, gb, partial, M, N, s);
+    case 64: return launch_layer_norm_grad<DT, PDT, 64>(gy, x, w, mean, rstd, gx, gw, gb, partial, M, N, s);
+    case 128: return launch_layer_norm_grad<DT, PDT, 128>(gy, x, w, mean, rstd, gx, gw, gb, partial, M, N, s);
+    case 256: return launch_layer_norm_grad<DT, PDT, 256>(gy, x, w, mean, rstd, gx, gw, gb, partial, M, N, s);
+    case 512: return launch_layer_norm_grad<DT, PDT, 512>(gy, x, w, mean, rstd, gx, gw, gb, partial, M, N, s);
+    default: return launch_layer_norm_grad<DT, PDT, 1024>(gy, x, w, mean, rstd, gx, gw, gb, partial, M, N, s);
     }
 }
 
@@ -811,7 +976,8 @@ REPDL_API int repdl_hip_layer_norm_grad(const void *grad_y, const void *x, const
     REPDL_REQUIRE(M == 0 || (grad_y != nullptr && x != nullptr && mean != nullptr && rstd != nullptr));
     hipStream_t s = repdl_stream(stream);
     float *partial = nullptr;
-    if (params && M > 0)
+    const bool one_launch = M > 0 && ln_few_rows(M, N);
+    if (params && M > 0 && !one_launch)
     {
         hipError_t e = repdl_ws_acquire(reinterpret_cast<void **>(&partial),
                                         (size_t)repdl_cdiv(M, ln_rows_per_block(M, N)) * 2 * (size_t)N * sizeof(float), s);
@@ -820,8 +986,8 @@ REPDL_API int repdl_hip_layer_norm_grad(const void *grad_y, const void *x, const
     }
     int rc = REPDL_OK;
     if (M > 0)
-        rc = LN_DISPATCH(dtype, param_dtype, layer_norm_grad_typed, grad_y, x, weight, mean, rstd, grad_x, partial, M, N, s);
-    if (rc == REPDL_OK && params)
+        rc = LN_DISPATCH(dtype, param_dtype, layer_norm_grad_typed, grad_y, x, weight, mean, rstd, grad_x, grad_weight, grad_bias, partial, M, N, s);
+    if (rc == REPDL_OK && params && !one_launch)
         rc = param_dtype == REPDL_F32    ? layer_norm_params<REPDL_F32>(partial, grad_weight, grad_bias, M, N, s)
              : param_dtype == REPDL_BF16 ? layer_norm_params<REPDL_BF16>(partial, grad_weight, grad_bias, M, N, s)
                                          : layer_norm_params<REPDL_F16>(partial, grad_weight, grad_bias, M, N, s);

@@ -5,7 +5,8 @@ A row of N elements belongs to T = 4, 8, ... 1024 threads, the fewest that hold 
 allows, and leaves out what an earlier one has.  A granule is summed in pairs and pairs of pairs, a thread's granules in turn,
 the threads of a wave (64) as a butterfly, the waves in turn.  Sums over rows: runs of consecutive rows, one per workgroup; inside a
 run the workgroup's teams take the rows in turn and their sums are added in the teams' order; then 16 sums of every 16th run are
-added in order.  (Rows of at most 16384 elements.)"""
+added in order.  At most 256 rows: one sixteenth of the workgroup's threads as many sums, each of every so-many-th row in turn, added
+in order.  (Rows of at most 16384 elements.)"""
 import numpy as np
 
 f32 = np.float32
@@ -60,6 +61,12 @@ class LayerNorm:
 
     def over_rows(self, v):
         threads = max(256, self.threads)
+        if self.rows <= 256:
+            groups = threads // 16
+            parts = np.zeros((groups, self.cols), f32)
+            for r in range(self.rows):
+                parts[r % groups] = (parts[r % groups] + v[r]).astype(f32)
+            return _in_turn(parts, 0)
         teams = threads // self.threads
         run = -(-self.rows // (512 if self.threads < 512 else 256))
         run = -(-run // teams) * teams

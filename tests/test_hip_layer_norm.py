@@ -74,6 +74,7 @@ def check_backward(got, x, w, b, gy, eps=1e-5):
         err = (got[0].double().cpu() - gx).abs()
         assert (err <= tol).all(), (float((err / tol).max()), x.shape, x.dtype)
     # sums over rows: at most rows / 512 (+ the teams of a workgroup) + 64 + 64 additions deep, each off by U of the sum of magnitudes
+    # (up to 256 rows: at most 16 rows and 64 sums)
     d = rows // 512 + 64 + 48 + 16
     for t, want, terms, extra in ((got[1], gw, gyd.abs() * xh.abs(), (gyd.abs() * xerr).sum(0)), (got[2], gb, gyd.abs(), 0.0)):
         if t is not None:
@@ -249,7 +250,8 @@ def test_refusals():
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 @pytest.mark.parametrize("shape", [(1, 1), (70, 3), (300, 7), (5, 8), (600, 20), (2000, 63), (37, 64), (1300, 100), (700, 1000), (40, 1025), (9, 2048), (600, 4100),
-                                   (5, 8191), (300, 16384)], ids=str)
+                                   (5, 8191), (300, 16384), (256, 3), (257, 3), (255, 130), (256, 1000), (257, 1000), (100, 4099), (256, 5000), (64, 16384), (1, 777)],
+                         ids=str)
 def test_bits_of_the_documented_order(shape, kind):
     """Outputs, statistics and all three gradients against a model of the sums' order in numpy's binary32: every bit."""
     from repdl_amd import ops
@@ -311,7 +313,7 @@ def test_entry_points_with_the_librarys_scratch():
 
     from repdl_amd import _lib, ops
 
-    x, w, b, gy = data(500, 300, torch.float32, torch.float32, seed=130)
+    x, w, b, gy = data(500, 300, torch.float32, torch.float32, seed=130)  # (more than 256 rows: with scratch)
     _, mean, rstd = ops.layer_norm(x, (300,), w, b)
     want = ops.layer_norm_grad(gy, x, mean, rstd, (300,), w)
     got = [torch.empty_like(t) for t in want]

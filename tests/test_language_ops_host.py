@@ -30,12 +30,13 @@ def test_layer_norm_arguments():
     assert lib.repdl_hip_layer_norm(None, None, None, None, None, None, 0, 8, 1e-5, 0, 0, None) == 0
     assert lib.repdl_hip_layer_norm(None, None, None, None, None, None, 4, 0, 1e-5, 0, 0, None) == 0
     assert lib.repdl_hip_layer_norm_grad(None, A, A, A, A, A, A, A, 4, 8, 0, 0, None) == -1
-    assert lib.repdl_hip_layer_norm_grad_ws(A, A, A, A, A, A, A, A, 4, 8, 0, 0, None, 0, None) == -3
-    assert lib.repdl_hip_layer_norm_grad_ws(A, A, A, A, A, A, A, A, 4, 8, 0, 0, A, 16, None) == -3
+    assert lib.repdl_hip_layer_norm_grad_ws(A, A, A, A, A, A, A, A, 400, 8, 0, 0, None, 0, None) == -3
+    assert lib.repdl_hip_layer_norm_grad_ws(A, A, A, A, A, A, A, A, 400, 8, 0, 0, A, 16, None) == -3
     assert lib.repdl_hip_layer_norm_grad_ws(A, A, A, A, A, None, None, None, 4, 8, 0, 0, None, 0, None) == 0  # nothing is wanted
     need = lib.repdl_hip_layer_norm_grad_workspace_bytes
     assert need(0, 8) == 0 and need(8, 0) == 0 and need(-1, 8) == 0
-    for rows, cols in ((1, 1), (100, 1000), (8192, 1024), (100000, 20000)):
+    assert need(1, 1) == 0 and need(256, 16384) == 0  # few rows: one launch, no partial sums
+    for rows, cols in ((1, 20000), (257, 1000), (8192, 1024), (100000, 20000)):
         assert 8 * cols <= need(rows, cols) <= 512 * 8 * cols + 512 and need(rows, cols) == need(rows, cols)
 
 
