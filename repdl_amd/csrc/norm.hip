@@ -846,14 +846,16 @@ int layer_norm_typed(const void *x, const void *w, const void *b, void *y, float
     }
 }
 
-// Runs of rows of the backward pass, each a multiple of the workgroup's teams: at most two of 256 threads to a CU, one of 512 or
-// 1024.  More cost more partial sums than they hide latency (512 against 256 runs, 4096 x 16384 bf16: 0.114 -> 0.101 ms; 1024 against
-// 512, 2048 x 2048: 0.0174 -> 0.0215), fewer leave CUs idle.
+// Runs of rows of the backward pass, each of at least four rows and a multiple of the workgroup's teams: 256 runs, one to a CU,
+// or 512 of 256 threads from 4096 rows on.  More runs write and read more partial sums, fewer leave a row's latency uncovered
+// (512 x 4096 bf16 in runs of 1 / 4 / 8 rows 0.0159 / 0.0116 / 0.0152 ms; 2048 x 2048 in 512 / 256 runs 0.0160 / 0.0135; 4096 x 16384
+// 0.114 / 0.101; 8192 x 4096 0.050 / 0.062).
 int64_t ln_rows_per_block(int64_t M, int64_t N)
 {
     const int tpr = N > LN_MAX_ONCHIP ? LN_MAX_TPR : ln_threads_per_row(N, LN_E);
     const int64_t teams = ln_grad_threads(tpr) / tpr;
-    return repdl_cdiv(repdl_cdiv(M, tpr < 512 ? 512 : 256), teams) * teams;
+    const int64_t rows = repdl_cdiv(M, tpr < 512 && M >= 4096 ? 512 : 256);
+    return repdl_cdiv(rows < 4 ? 4 : rows, teams) * teams;
 }
 
 // Rows up to which one launch makes all gradients (layer_norm_grad_few_kernel).  Both sides, two launches against one: 64 x 1024 f32

@@ -68,7 +68,7 @@ class LayerNorm:
                 parts[r % groups] = (parts[r % groups] + v[r]).astype(f32)
             return _in_turn(parts, 0)
         teams = threads // self.threads
-        run = -(-self.rows // (512 if self.threads < 512 else 256))
+        run = max(4, -(-self.rows // (512 if self.threads < 512 and self.rows >= 4096 else 256)))
         run = -(-run // teams) * teams
         runs = []
         for r0 in range(0, self.rows, run):
