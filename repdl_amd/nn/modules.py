@@ -66,7 +66,8 @@ class Dropout(torch.nn.Dropout):
     ``rng_state`` (int64: seed, number of the next call) is a buffer that moves with the module and, like everything of
     ``torch.nn.Dropout``, is not part of the state_dict: save it beside the weights to go on with the masks of an
     interrupted run.  ``seed`` (in [0, 2^63)) defaults to a draw from PyTorch's CPU generator.  A layer that is copied
-    (``copy.deepcopy``) draws the same masks as its original: give copies that are to differ a seed of their own.
+    (``copy.deepcopy``) draws the same masks as its original: give copies that are to differ a seed of their own.  The call
+    number goes up on the device: calls of one layer on several streams at once need an order between them.
     Recomputing a forward pass (activation checkpointing) takes another call and so another mask: use
     ``functional.dropout`` with the state of the first one there.
     ``forward(input, residual)`` adds the residual in the same pass."""

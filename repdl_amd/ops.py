@@ -202,6 +202,8 @@ def _dropout_state(state: Union[torch.Tensor, Tuple[int, int]]) -> Tuple[Optiona
     """(tensor, 0, 0) or (None, seed, call), as the backend takes it."""
     if isinstance(state, torch.Tensor):
         return state, 0, 0
+    if not isinstance(state, (tuple, list)) or len(state) != 2:
+        raise TypeError("dropout: the state is an int64 tensor (seed, call) or two integers, got %r" % (state,))
     seed, call = (int(v) for v in state)
     if not (0 <= seed < 2 ** 64 and 0 <= call < 2 ** 64):
         raise ValueError("dropout: seed and call are integers in [0, 2^64)")

@@ -53,6 +53,9 @@ def test_dropout_arguments():
     assert lib.repdl_hip_dropout_next_call(None, A, None) == -1
     with pytest.raises(ValueError):
         F.dropout(torch.zeros(3), 1.5, (1, 2))
+    for state in (True, None, 3, (1, 2, 3)):  # (what torch's third argument would be, among others)
+        with pytest.raises(TypeError):
+            ops._dropout_state(state)
     x = torch.zeros(3)
     assert F.dropout(x, 0.5, (1, 2), training=False) is x
 
