@@ -14,10 +14,12 @@
 //   over rows    a workgroup's run of rows, each of its teams taking every (number of teams)-th one in turn; the teams in turn; sixteen
 //                sums of every sixteenth run; those in turn.  At most 256 rows: 16 to 64 sums of every 16th to 64th row, those in turn.
 //
-// The two passes over a row (mean, then centred squares) read it from registers: one thread holds E = 16 of its elements, as
+// The two passes over a row (mean, then centred squares) read it from registers: one thread holds E = 16 or 24 of its elements, as
 // 16-byte granules TPR granules apart, TPR threads a row.  Bound: HBM, 2 passes over the tensor forward and 3 backward.  Measured
 // (a copy of 1 GiB moves 5.1 TB/s): forward 16384 x 8192 bf16 0.094 ms = 5.7 TB/s, 8192 x 1024 f32 0.0130 = 5.2, 65536 x 256 f32
 // 0.027 = 5.0; backward with both launches 0.166 ms = 4.8 TB/s, 0.026 = 3.8, 0.048 = 4.2.
+#include <type_traits>
+
 #include "lowp.h"
 #include "crmath.h"
 #include "lanes.h"
@@ -32,10 +34,20 @@ __host__ __device__ constexpr int ln_threads_per_row(int64_t N, int E)
         t *= 2;
     return t;
 }
-constexpr int LN_E = 16;
 constexpr int ln_grad_threads(int tpr) { return tpr < 256 ? 256 : tpr; }
-constexpr int LN_MAX_TPR = 1024; // rows of more than LN_MAX_TPR * LN_E elements are read from memory for every pass
-constexpr int64_t LN_MAX_ONCHIP = (int64_t)LN_MAX_TPR * LN_E;
+constexpr int64_t LN_MAX_ONCHIP = 16384; // (1024 threads of 16 elements; longer rows are read from memory for every pass)
+
+// Elements per thread: 16, or 24 in a 16-bit type whose row would leave many of 16 elements' threads without any (half the threads
+// then hold it).  Forward wherever that pads the row less, rows of up to 1.5 powers of two: 32768 x 2056 f16 0.0696 -> 0.0535 ms,
+// 32768 x 1280 bf16 0.0389 -> 0.0351, 32768 x 1536 0.0405 -> 0.0401.  Backward, where a thread's sums of gw and gb grow with its elements,
+// for rows of up to 1.125 powers of two: 2056 0.111 -> 0.090, 1280 0.0604 -> 0.0581, but 8192 x 5120 0.0561 -> 0.0604.
+int ln_elements(int64_t N, int dtype, bool backward)
+{
+    const int64_t padded = 16 * (int64_t)ln_threads_per_row(N, 16);
+    if (dtype == REPDL_F32 || padded <= 64 || N > LN_MAX_ONCHIP)
+        return 16;
+    return backward ? (16 * N <= 9 * padded ? 24 : 16) : (4 * N <= 3 * padded ? 24 : 16);
+}
 
 // Sum over the TPR threads of a row of K values each, in every thread of the row: a butterfly inside the wave, then the
 // waves' sums in order.  `scratch`: K * (TPR / 64) floats of LDS per row team, free again at the next call's second barrier;
@@ -798,7 +810,25 @@ bool ln_streams(int64_t M, int64_t N, const void *out)
     return M * N >= REPDL_STREAM_BYTES / repdl_dtype_bytes(DT) && N % Lowp<DT>::G == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
 }
 
-template <int DT, int PDT, int TPR, bool TINY = false>
+// f(threads per row as a constant) for rows of `tpr` threads
+template <typename F>
+int ln_with_threads(int tpr, F f)
+{
+    switch (tpr)
+    {
+    case 4: return f(std::integral_constant<int, 4>());
+    case 8: return f(std::integral_constant<int, 8>());
+    case 16: return f(std::integral_constant<int, 16>());
+    case 32: return f(std::integral_constant<int, 32>());
+    case 64: return f(std::integral_constant<int, 64>());
+    case 128: return f(std::integral_constant<int, 128>());
+    case 256: return f(std::integral_constant<int, 256>());
+    case 512: return f(std::integral_constant<int, 512>());
+    default: return f(std::integral_constant<int, 1024>());
+    }
+}
+
+template <int DT, int PDT, int TPR, int E, bool TINY>
 int launch_layer_norm(const void *x, const void *w, const void *b, void *y, float *mean, float *rstd, int64_t M, int64_t N, float eps,
                       hipStream_t s)
 {
@@ -807,11 +837,11 @@ int launch_layer_norm(const void *x, const void *w, const void *b, void *y, floa
     constexpr int THREADS = TPR < 256 ? 256 : TPR, TEAMS = THREADS / TPR;
     const dim3 grid((unsigned)repdl_cdiv(M, TEAMS));
     if (TPR >= 64 && ln_streams<DT>(M, N, y))
-        REPDL_LAUNCH((layer_norm_kernel<DT, PDT, TPR, LN_E, TINY, (TPR >= 64)>), grid, dim3(THREADS), 0, s, static_cast<const T *>(x),
+        REPDL_LAUNCH((layer_norm_kernel<DT, PDT, TPR, E, TINY, (TPR >= 64)>), grid, dim3(THREADS), 0, s, static_cast<const T *>(x),
                      static_cast<const P *>(w), static_cast<const P *>(b), static_cast<T *>(y), mean, rstd, M, (int)N,
                      (float)(1.0 / (double)N), eps);
     else
-        REPDL_LAUNCH((layer_norm_kernel<DT, PDT, TPR, LN_E, TINY, false>), grid, dim3(THREADS), 0, s, static_cast<const T *>(x),
+        REPDL_LAUNCH((layer_norm_kernel<DT, PDT, TPR, E, TINY, false>), grid, dim3(THREADS), 0, s, static_cast<const T *>(x),
                      static_cast<const P *>(w), static_cast<const P *>(b), static_cast<T *>(y), mean, rstd, M, (int)N,
                      (float)(1.0 / (double)N), eps);
     return repdl_launch_status();
@@ -831,28 +861,23 @@ int layer_norm_typed(const void *x, const void *w, const void *b, void *y, float
         return repdl_launch_status();
     }
     if (N < Lowp<DT>::G)
-        return launch_layer_norm<DT, PDT, 4, true>(x, w, b, y, mean, rstd, M, N, eps, s);
-    switch (ln_threads_per_row(N, LN_E))
-    {
-    case 4: return launch_layer_norm<DT, PDT, 4>(x, w, b, y, mean, rstd, M, N, eps, s);
-    case 8: return launch_layer_norm<DT, PDT, 8>(x, w, b, y, mean, rstd, M, N, eps, s);
-    case 16: return launch_layer_norm<DT, PDT, 16>(x, w, b, y, mean, rstd, M, N, eps, s);
-    case 32: return launch_layer_norm<DT, PDT, 32>(x, w, b, y, mean, rstd, M, N, eps, s);
-    case 64: return launch_layer_norm<DT, PDT, 64>(x, w, b, y, mean, rstd, M, N, eps, s);
-    case 128: return launch_layer_norm<DT, PDT, 128>(x, w, b, y, mean, rstd, M, N, eps, s);
-    case 256: return launch_layer_norm<DT, PDT, 256>(x, w, b, y, mean, rstd, M, N, eps, s);
-    case 512: return launch_layer_norm<DT, PDT, 512>(x, w, b, y, mean, rstd, M, N, eps, s);
-    default: return launch_layer_norm<DT, PDT, 1024>(x, w, b, y, mean, rstd, M, N, eps, s);
-    }
+        return launch_layer_norm<DT, PDT, 4, 16, true>(x, w, b, y, mean, rstd, M, N, eps, s);
+    const int E = ln_elements(N, DT, false);
+    return ln_with_threads(ln_threads_per_row(N, E), [&](auto threads) {
+        constexpr int TPR = decltype(threads)::value;
+        constexpr int E24 = DT == REPDL_F32 || TPR == 1024 ? 16 : 24; // (no such rows of binary32, nor of 1024 threads)
+        return E == 24 ? launch_layer_norm<DT, PDT, TPR, E24, false>(x, w, b, y, mean, rstd, M, N, eps, s)
+                       : launch_layer_norm<DT, PDT, TPR, 16, false>(x, w, b, y, mean, rstd, M, N, eps, s);
+    });
 }
 
 // Runs of rows of the backward pass, each of at least four rows and a multiple of the workgroup's teams: 256 runs, one to a CU,
 // or 512 of 256 threads from 4096 rows on.  More runs write and read more partial sums, fewer leave a row's latency uncovered
 // (512 x 4096 bf16 in runs of 1 / 4 / 8 rows 0.0159 / 0.0116 / 0.0152 ms; 2048 x 2048 in 512 / 256 runs 0.0160 / 0.0135; 4096 x 16384
 // 0.114 / 0.101; 8192 x 4096 0.050 / 0.062).
-int64_t ln_rows_per_block(int64_t M, int64_t N)
+int64_t ln_rows_per_block(int64_t M, int64_t N, int dtype)
 {
-    const int tpr = N > LN_MAX_ONCHIP ? LN_MAX_TPR : ln_threads_per_row(N, LN_E);
+    const int tpr = N > LN_MAX_ONCHIP ? 1024 : ln_threads_per_row(N, ln_elements(N, dtype, true));
     const int64_t teams = ln_grad_threads(tpr) / tpr;
     const int64_t rows = repdl_cdiv(M, tpr < 512 && M >= 4096 ? 512 : 256);
     return repdl_cdiv(rows < 4 ? 4 : rows, teams) * teams;
@@ -864,7 +889,7 @@ int64_t ln_rows_per_block(int64_t M, int64_t N)
 constexpr int64_t LN_FEW_ROWS = 256;
 bool ln_few_rows(int64_t M, int64_t N) { return M <= LN_FEW_ROWS && N <= LN_MAX_ONCHIP; }
 
-template <int DT, int PDT, int TPR, bool TINY = false>
+template <int DT, int PDT, int TPR, int E, bool TINY>
 int launch_layer_norm_grad(const void *gy, const void *x, const void *w, const float *mean, const float *rstd, void *gx, void *gw, void *gb,
                            float *partial, int64_t M, int64_t N, hipStream_t s)
 {
@@ -874,19 +899,19 @@ int launch_layer_norm_grad(const void *gy, const void *x, const void *w, const f
     {
         const int rows = gx != nullptr ? (int)repdl_cdiv(M, ln_grad_threads(TPR) / TPR) : 0;
         const int cols = gw != nullptr || gb != nullptr ? (int)repdl_cdiv(N, 16 * Lowp<DT>::G) : 0;
-        REPDL_LAUNCH((layer_norm_grad_few_kernel<DT, PDT, TPR, LN_E, TINY>), dim3((unsigned)(rows + cols)), dim3(ln_grad_threads(TPR)), 0, s,
+        REPDL_LAUNCH((layer_norm_grad_few_kernel<DT, PDT, TPR, E, TINY>), dim3((unsigned)(rows + cols)), dim3(ln_grad_threads(TPR)), 0, s,
                      static_cast<const T *>(gy), static_cast<const T *>(x), static_cast<const P *>(w), mean, rstd, static_cast<T *>(gx),
                      static_cast<P *>(gw), static_cast<P *>(gb), (int)M, (int)N, rows, (float)(1.0 / (double)N));
         return repdl_launch_status();
     }
-    const int64_t rpb = ln_rows_per_block(M, N);
+    const int64_t rpb = ln_rows_per_block(M, N, DT);
     const dim3 grid((unsigned)repdl_cdiv(M, rpb)), block(ln_grad_threads(TPR));
     if (TPR >= 64 && ln_streams<DT>(M, N, gx))
-        REPDL_LAUNCH((layer_norm_grad_kernel<DT, PDT, TPR, LN_E, TINY, (TPR >= 64)>), grid, block, 0, s, static_cast<const T *>(gy),
+        REPDL_LAUNCH((layer_norm_grad_kernel<DT, PDT, TPR, E, TINY, (TPR >= 64)>), grid, block, 0, s, static_cast<const T *>(gy),
                      static_cast<const T *>(x), static_cast<const P *>(w), mean, rstd, static_cast<T *>(gx), partial, M, (int)N, rpb,
                      (float)(1.0 / (double)N));
     else
-        REPDL_LAUNCH((layer_norm_grad_kernel<DT, PDT, TPR, LN_E, TINY, false>), grid, block, 0, s, static_cast<const T *>(gy),
+        REPDL_LAUNCH((layer_norm_grad_kernel<DT, PDT, TPR, E, TINY, false>), grid, block, 0, s, static_cast<const T *>(gy),
                      static_cast<const T *>(x), static_cast<const P *>(w), mean, rstd, static_cast<T *>(gx), partial, M, (int)N, rpb,
                      (float)(1.0 / (double)N));
     return repdl_launch_status();
@@ -906,7 +931,7 @@ int layer_norm_grad_typed(const void *gy, const void *x, const void *w, const fl
                          (float)(1.0 / (double)N));
         if (partial != nullptr)
         {
-            const int64_t rpb = ln_rows_per_block(M, N);
+            const int64_t rpb = ln_rows_per_block(M, N, DT);
             REPDL_LAUNCH((layer_norm_param_long_kernel<DT>),
                          dim3((unsigned)repdl_cdiv(N, 256 * Lowp<DT>::G), (unsigned)repdl_cdiv(M, rpb)), dim3(256), 0, s,
                          static_cast<const T *>(gy), static_cast<const T *>(x), mean, rstd, partial, M, N, rpb);
@@ -914,27 +939,22 @@ int layer_norm_grad_typed(const void *gy, const void *x, const void *w, const fl
         return repdl_launch_status();
     }
     if (N < Lowp<DT>::G)
-        return launch_layer_norm_grad<DT, PDT, 4, true>(gy, x, w, mean, rstd, gx, gw, gb, partial, M, N, s);
-    switch (ln_threads_per_row(N, LN_E))
-    {
-    case 4: return launch_layer_norm_grad<DT, PDT, 4>(gy, x, w, mean, rstd, gx, gw, gb, partial, M, N, s);
-    case 8: return launch_layer_norm_grad<DT, PDT, 8>(gy, x, w, mean, rstd, gx, gw, gb, partial, M, N, s);
-    case 16: return launch_layer_norm_grad<DT, PDT, 16>(gy, x, w, mean, rstd, gx, gw, gb, partial, M, N, s);
-    case 32: return launch_layer_norm_grad<DT, PDT, 32>(gy, x, w, mean, rstd, gx, gw, gb, partial, M, N, s);
-    case 64: return launch_layer_norm_grad<DT, PDT, 64>(gy, x, w, mean, rstd, gx, gw, gb, partial, M, N, s);
-    case 128: return launch_layer_norm_grad<DT, PDT, 128>(gy, x, w, mean, rstd, gx, gw, gb, partial, M, N, s);
-    case 256: return launch_layer_norm_grad<DT, PDT, 256>(gy, x, w, mean, rstd, gx, gw, gb, partial, M, N, s);
-    case 512: return launch_layer_norm_grad<DT, PDT, 512>(gy, x, w, mean, rstd, gx, gw, gb, partial, M, N, s);
-    default: return launch_layer_norm_grad<DT, PDT, 1024>(gy, x, w, mean, rstd, gx, gw, gb, partial, M, N, s);
-    }
+        return launch_layer_norm_grad<DT, PDT, 4, 16, true>(gy, x, w, mean, rstd, gx, gw, gb, partial, M, N, s);
+    const int E = ln_elements(N, DT, true);
+    return ln_with_threads(ln_threads_per_row(N, E), [&](auto threads) {
+        constexpr int TPR = decltype(threads)::value;
+        constexpr int E24 = DT == REPDL_F32 || TPR == 1024 ? 16 : 24;
+        return E == 24 ? launch_layer_norm_grad<DT, PDT, TPR, E24, false>(gy, x, w, mean, rstd, gx, gw, gb, partial, M, N, s)
+                       : launch_layer_norm_grad<DT, PDT, TPR, 16, false>(gy, x, w, mean, rstd, gx, gw, gb, partial, M, N, s);
+    });
 }
 
 template <int PDT>
-int layer_norm_params(const float *partial, void *gw, void *gb, int64_t M, int64_t N, hipStream_t s)
+int layer_norm_params(const float *partial, void *gw, void *gb, int64_t M, int64_t N, int dtype, hipStream_t s)
 {
     typedef typename LowpType<PDT>::T P;
     // (no rows: no blocks, the sums of nothing)
-    const int blocks = M == 0 ? 0 : (int)repdl_cdiv(M, ln_rows_per_block(M, N));
+    const int blocks = M == 0 ? 0 : (int)repdl_cdiv(M, ln_rows_per_block(M, N, dtype));
     REPDL_LAUNCH((layer_norm_param_kernel<PDT>), dim3((unsigned)repdl_cdiv(2 * N, 64)), dim3(64 * LN_FOLD), 0, s, partial,
                  static_cast<P *>(gw), static_cast<P *>(gb), N, blocks);
     return repdl_launch_status();
@@ -982,7 +1002,7 @@ REPDL_API int repdl_hip_layer_norm_grad(const void *grad_y, const void *x, const
     if (params && M > 0 && !one_launch)
     {
         hipError_t e = repdl_ws_acquire(reinterpret_cast<void **>(&partial),
-                                        (size_t)repdl_cdiv(M, ln_rows_per_block(M, N)) * 2 * (size_t)N * sizeof(float), s);
+                                        (size_t)repdl_cdiv(M, ln_rows_per_block(M, N, dtype)) * 2 * (size_t)N * sizeof(float), s);
         if (e != hipSuccess)
             return (int)e;
     }
@@ -990,9 +1010,9 @@ REPDL_API int repdl_hip_layer_norm_grad(const void *grad_y, const void *x, const
     if (M > 0)
         rc = LN_DISPATCH(dtype, param_dtype, layer_norm_grad_typed, grad_y, x, weight, mean, rstd, grad_x, grad_weight, grad_bias, partial, M, N, s);
     if (rc == REPDL_OK && params && !one_launch)
-        rc = param_dtype == REPDL_F32    ? layer_norm_params<REPDL_F32>(partial, grad_weight, grad_bias, M, N, s)
-             : param_dtype == REPDL_BF16 ? layer_norm_params<REPDL_BF16>(partial, grad_weight, grad_bias, M, N, s)
-                                         : layer_norm_params<REPDL_F16>(partial, grad_weight, grad_bias, M, N, s);
+        rc = param_dtype == REPDL_F32    ? layer_norm_params<REPDL_F32>(partial, grad_weight, grad_bias, M, N, dtype, s)
+             : param_dtype == REPDL_BF16 ? layer_norm_params<REPDL_BF16>(partial, grad_weight, grad_bias, M, N, dtype, s)
+                                         : layer_norm_params<REPDL_F16>(partial, grad_weight, grad_bias, M, N, dtype, s);
     if (partial != nullptr)
     {
         const hipError_t e = repdl_ws_release(partial, s);
@@ -1007,7 +1027,14 @@ REPDL_API size_t repdl_hip_layer_norm_grad_workspace_bytes(int64_t M, int64_t N)
     if (!ln_shape_ok(M, N, REPDL_F32, REPDL_F32) || M == 0 || N == 0)
         return 0;
     float *fake = const_cast<float *>(repdl_ws_fake_pointer(true));
-    return repdl_ws_query([&]() { return repdl_hip_layer_norm_grad(fake, fake, fake, fake, fake, fake, fake, fake, M, N, REPDL_F32, REPDL_F32, nullptr); });
+    size_t need = 0; // (for any type: the runs of rows of binary32 and of 16 bits may differ)
+    for (int dtype : {REPDL_F32, REPDL_BF16})
+    {
+        const size_t bytes =
+            repdl_ws_query([&]() { return repdl_hip_layer_norm_grad(fake, fake, fake, fake, fake, fake, fake, fake, M, N, dtype, REPDL_F32, nullptr); });
+        need = bytes > need ? bytes : need;
+    }
+    return need;
 }
 
 REPDL_API int repdl_hip_layer_norm_grad_ws(const void *grad_y, const void *x, const void *weight, const float *mean, const float *rstd,

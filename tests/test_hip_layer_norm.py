@@ -149,11 +149,12 @@ def test_gradients_against_differences():
         assert abs(float((g.double().cpu() * v).sum()) - want) <= size * 100 * U + 1e-6
 
 
-@pytest.mark.parametrize("cols", [5, 64, 1000, 4096, 9000])
-def test_rows_do_not_depend_on_their_batch(cols):
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("cols", [5, 64, 1000, 1100, 1280, 4096, 9000])
+def test_rows_do_not_depend_on_their_batch(cols, kind):
     from repdl_amd import ops
 
-    x, w, b, gy = data(300, cols, torch.float32, torch.float32, seed=60)
+    x, w, b, gy = data(300, cols, TYPES[kind], torch.float32, seed=60)
     y, mean, rstd = ops.layer_norm(x, (cols,), w, b)
     gx = ops.layer_norm_grad(gy, x, mean, rstd, (cols,), w)[0]
     for at, n in ((0, 1), (7, 1), (100, 64), (299, 1)):
@@ -251,7 +252,8 @@ def test_refusals():
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 @pytest.mark.parametrize("shape", [(1, 1), (70, 3), (300, 7), (5, 8), (600, 20), (2000, 63), (37, 64), (1300, 100), (700, 1000), (40, 1025), (9, 2048), (600, 4100),
                                    (5, 8191), (300, 16384), (256, 3), (257, 3), (255, 130), (256, 1000), (257, 1000), (100, 4099), (256, 5000), (64, 16384), (1, 777), (4095, 200),
-                                   (4096, 200), (4100, 65), (1100, 5000), (4200, 8200)],
+                                   (4096, 200), (4100, 65), (1100, 5000), (4200, 8200), (50, 64), (50, 65), (300, 72), (300, 73), (50, 96), (50, 97), (300, 144),
+                                   (300, 145), (40, 1152), (40, 1153), (300, 1280), (40, 1536), (40, 1537), (300, 2050), (4500, 2056), (20, 9216), (20, 12288), (20, 12289)],
                          ids=str)
 def test_bits_of_the_documented_order(shape, kind):
     """Outputs, statistics and all three gradients against a model of the sums' order in numpy's binary32: every bit."""
@@ -270,7 +272,7 @@ def test_bits_of_the_documented_order(shape, kind):
 
 
 @pytest.mark.parametrize("kind", sorted(TYPES))
-@pytest.mark.parametrize("cols", [1000, 2048, 4096, 8192, 16384])
+@pytest.mark.parametrize("cols", [1000, 1280, 2048, 2056, 4096, 8192, 16384])
 def test_large_tensors_have_the_bits_of_their_parts(kind, cols):
     """256 MB and more are moved past the caches, by other instructions."""
     from repdl_amd import ops
