@@ -19,7 +19,8 @@ def reference(logits, target, ref, beta, eps, ignore=-100):
     x = logits.detach().double().cpu()
     t = target.cpu()
     counted = t != ignore
-    lse = torch.logsumexp(x, 2)
+    x = x - x.amax(2, keepdim=True)  # (exact enough in binary64; a large logit minus its logsumexp would lose the logarithm)
+    lse = torch.log(torch.exp(x).sum(2))
     lp = x.gather(2, t.clamp(min=0).unsqueeze(2)).squeeze(2) - lse
     logps = torch.where(counted, lp, 0.0).sum(1)
     P = len(x) // 2
@@ -202,6 +203,19 @@ def test_masked_vocabulary_and_large_logits(vocab, kind):
     big = (x.float() * 0 + 1000.0 + 3 * gen.normal_like(65, *x.shape).cuda()).to(TYPES[kind]).requires_grad_()
     loss, logps = F.preference_loss(big, t, ref)
     check(loss, logps, torch.autograd.grad(loss, big)[0], big, t, ref, 0.1, 0.0)
+
+
+@pytest.mark.parametrize("kind", sorted(TYPES))
+@pytest.mark.parametrize("vocab", [40, 3000, 20000])
+def test_rows_of_one_value(vocab, kind):
+    """Every logit the same -- the type's lowest value, its largest, 0 --: each token has probability 1 / V."""
+    from repdl_amd.nn import functional as F
+
+    t = gen.labels(66, 4, vocab).view(2, 2).cuda()
+    for value in (torch.finfo(TYPES[kind]).min, torch.finfo(TYPES[kind]).max, 0.0, -3.0e4, 2.0 ** 21 if kind != "f16" else 2.0 ** 15):
+        y = torch.full((2, 2, vocab), value, dtype=TYPES[kind], device="cuda", requires_grad=True)
+        loss, logps = F.preference_loss(y, t)
+        check(loss, logps, torch.autograd.grad(loss, y)[0], y, t, None, 0.1, 0.0)
 
 
 @pytest.mark.parametrize("vocab", [50, 3000, 20000])
