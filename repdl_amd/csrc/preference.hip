@@ -332,6 +332,9 @@ __global__ __launch_bounds__(256, 4) void preference_grad_kernel(const typename 
     const int64_t c1 = c0 + p.width < p.vocab ? c0 + p.width : p.vocab;
     const int width = (int)(c1 - c0);
     typename L::T *gr = gx + (int64_t)row * p.vocab + c0;
+    // (read beside the target that decides whether they count: one trip to memory instead of two)
+    const float2 st = row_stats[row];
+    const float cc = coef[row / (uint32_t)p.steps] * *grad_loss;
     const int64_t t = target[row];
     float v[G];
     if (t == p.ignore)
@@ -357,8 +360,6 @@ __global__ __launch_bounds__(256, 4) void preference_grad_kernel(const typename 
         if (c + G <= width)
             raw[i] = L::template load_raw<STREAM>(xr + c);
     }
-    const float2 st = row_stats[row];
-    const float cc = coef[row / (uint32_t)p.steps] * *grad_loss;
     const float k0 = -(cc * st.y);
     const int64_t at = t - c0; // the target's column in this chunk, if it has it
 #pragma unroll
