@@ -29,7 +29,13 @@ struct LowpType<REPDL_F16>
 {
     typedef _Float16 T;
     __device__ static __forceinline__ float widen(_Float16 v) { return (float)v; }
-    __device__ static __forceinline__ _Float16 narrow(float v) { return (_Float16)v; }
+    __device__ static __forceinline__ _Float16 narrow(float v)
+    {
+        // The value as binary32 has it, then the conversion: left to itself the compiler makes one v_fma_mixlo_f16 of a product and the
+        // conversion where it packs no pair, which rounds once -- and the same element differs with its place in the tensor.
+        asm("" : "+v"(v));
+        return (_Float16)v;
+    }
 };
 
 // Tensors of this size and more are read and written past the caches (non-temporal accesses): what a kernel leaves of a smaller

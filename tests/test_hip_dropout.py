@@ -35,6 +35,21 @@ def test_mask_and_values(n, kind):
             assert abs(int((~keep).sum()) - n * p) <= 6 * (n * p * (1 - p)) ** 0.5
 
 
+@pytest.mark.parametrize("n", [8, 4096, 4097, 4099, 4103])
+def test_two_roundings_in_float16_everywhere(n):
+    """A product whose rounding to binary32 lies half way between two float16 numbers: the second rounding then goes to the even
+    one, at the end of a tensor (element by element) as inside (in granules)."""
+    from repdl_amd import ops
+
+    p = 0.7500858221038925  # 0.7109375 * float(1 / (1 - p)) rounds to 2.8447265625, half way between 2.84375 and 2.845703125
+    x = torch.full((n,), 0.7109375, dtype=torch.float16)
+    want, keep = expected(x, p, 3, 4)
+    assert keep[-8:].any() and set(want[keep].tolist()) == {2.84375}
+    assert torch.equal(ops.dropout(x.cuda(), p, (3, 4)).cpu(), want)
+    for at in range(n - 8, n):  # the same element as the last one
+        assert torch.equal(ops.dropout(x[:at + 1].cuda(), p, (3, 4)).cpu(), want[:at + 1])
+
+
 def test_known_answers():
     """Three blocks of the generator from the paper's reference vectors, as masks: word >= round(p 2^32) at thresholds on
     either side of each word."""

@@ -249,7 +249,7 @@ def test_refusals():
             call()
 
 
-@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("shape", [(1, 1), (70, 3), (300, 7), (5, 8), (600, 20), (2000, 63), (37, 64), (1300, 100), (700, 1000), (40, 1025), (9, 2048), (600, 4100),
                                    (5, 8191), (300, 16384), (256, 3), (257, 3), (255, 130), (256, 1000), (257, 1000), (100, 4099), (256, 5000), (64, 16384), (1, 777), (4095, 200),
                                    (4096, 200), (4100, 65), (1100, 5000), (4200, 8200), (50, 64), (50, 65), (300, 72), (300, 73), (50, 96), (50, 97), (300, 144),
