@@ -91,6 +91,51 @@ def test_against_the_definition(case, kind):
         assert torch.equal(alone[0], loss.detach()) and torch.equal(alone[1], logps)
 
 
+@pytest.fixture(scope="module")
+def model(tmp_path_factory):
+    """preference_model.c as a function of tensors -> loss, logps, row statistics, coefficients"""
+    import ctypes
+    import os
+    import subprocess
+
+    here = os.path.dirname(os.path.abspath(__file__))
+    so = str(tmp_path_factory.mktemp("model") / "preference_model.so")
+    subprocess.run(["gcc", "-O2", "-std=c11", "-ffp-contract=off", "-mfma", "-shared", "-fPIC", "-I", os.path.join(here, "..", "repdl_amd", "csrc"),
+                    os.path.join(here, "preference_model.c"), "-o", so, "-lm"], check=True)
+    lib = ctypes.CDLL(so)
+    i64, f64 = ctypes.c_int64, ctypes.c_double
+
+    def run(x, t, ref, beta, eps, ignore=-100):
+        seqs, steps, vocab = x.shape
+        xc, tc = x.detach().float().cpu().contiguous(), t.cpu().contiguous()
+        rc = None if ref is None else ref.cpu()
+        out = [torch.zeros(()), torch.zeros(seqs), torch.zeros(seqs, steps, 2), torch.zeros(seqs)]
+        p = lambda v: None if v is None else ctypes.c_void_p(v.data_ptr())  # noqa: E731
+        lib.preference_model(p(xc), p(tc), p(rc), i64(seqs // 2), i64(steps), i64(vocab), 4 if x.dtype == torch.float32 else 8, f64(beta), f64(eps),
+                             i64(ignore), *(p(v) for v in out))
+        return out
+
+    return run
+
+
+@pytest.mark.parametrize("kind", sorted(TYPES))
+@pytest.mark.parametrize("case", CASES + [(1, 700, 70), (3, 2, 40000), (1100, 1, 5), (1, 2, 131072)], ids=str)
+def test_bits_of_the_documented_order(case, kind, model):
+    from repdl_amd import ops
+
+    x, t, ref = data(*case, kind, seed=33)
+    for r, beta, eps in ((ref, 0.1, 0.0), (None, 0.5, 0.2)):
+        got = ops.preference_loss(x, t, r, beta, eps)
+        for g, want in zip(got, model(x, t, r, beta, eps)):
+            g = g.cpu()
+            if g.dim() == 3:  # (the statistics of a token that is not counted are not read)
+                g, want = g[t.cpu() != -100], want[t.cpu() != -100]
+            assert torch.equal(g.view(torch.int32), want.view(torch.int32))
+    far = (x.float() * 0.5 - 3.0e6).to(x.dtype) if kind != "f16" else x - 6.0e4  # (beyond the terms' integers: the maximum subtracted first)
+    got, want = ops.preference_loss(far, t, ref), model(far, t, ref, 0.1, 0.0)
+    assert torch.equal(got[1].cpu(), want[1]) and torch.equal(got[0].cpu(), want[0])
+
+
 def test_incoming_gradient_scales():
     from repdl_amd.nn import functional as F
 
