@@ -592,6 +592,24 @@ variable_list once(variable_list grads)
     return (*error)(std::move(grads));
 }
 
+// A leaf's gradient accumulator belongs to the stream of the first graph that used the leaf, for as long as a graph of it lives.
+// If that is the default stream, a backward pass through the leaf under capture makes the default stream wait for an event of the
+// capture, which ends the process inside PyTorch's engine.  Said here, in the forward pass, where it can still be an error.
+void refuse_eager_leaf(const torch::Tensor &t, const char *name)
+{
+    if (!at::GradMode::is_enabled() || !t.defined() || !t.is_cuda() || !t.requires_grad() || !t.is_leaf())
+        return;
+    const auto current = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index());
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (current.stream() == nullptr || hipStreamIsCapturing(current.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone)
+        return;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+    const auto held = node ? node->stream() : c10::nullopt;
+    TORCH_CHECK(!held.has_value() || *held != c10::Stream(c10::Stream::DEFAULT, t.device()), name,
+                " still belongs to an eager graph of the default stream: a backward pass cannot be captured beside it; delete the eager "
+                "graph's results first (or run the eager steps on a side stream)");
+}
+
 struct LayerNormFunction : public torch::autograd::Function<LayerNormFunction>
 {
     static torch::Tensor forward(AutogradContext *ctx, const torch::Tensor &x, const c10::optional<torch::Tensor> &weight,
@@ -686,12 +704,20 @@ struct PreferenceFunction : public torch::autograd::Function<PreferenceFunction>
 torch::Tensor layer_norm_autograd(const torch::Tensor &input, int64_t n, const c10::optional<torch::Tensor> &weight,
                                   const c10::optional<torch::Tensor> &bias, double eps)
 {
+    refuse_eager_leaf(input, "input");
+    if (weight.has_value())
+        refuse_eager_leaf(*weight, "weight");
+    if (bias.has_value())
+        refuse_eager_leaf(*bias, "bias");
     return LayerNormFunction::apply(input, weight, bias, n, eps);
 }
 
 torch::Tensor dropout_autograd(const torch::Tensor &input, const c10::optional<torch::Tensor> &residual, double p,
                                const c10::optional<torch::Tensor> &state, uint64_t seed, uint64_t call)
 {
+    refuse_eager_leaf(input, "input");
+    if (residual.has_value())
+        refuse_eager_leaf(*residual, "residual");
     return DropoutFunction::apply(input, residual, p, state, (int64_t)seed, (int64_t)call);
 }
 
@@ -699,6 +725,7 @@ std::tuple<torch::Tensor, torch::Tensor> preference_loss_autograd(const torch::T
                                                                   const c10::optional<torch::Tensor> &ref_logps, double beta,
                                                                   double label_smoothing, int64_t ignore_index)
 {
+    refuse_eager_leaf(logits, "logits");
     auto r = PreferenceFunction::apply(logits, target, ref_logps, beta, label_smoothing, ignore_index);
     return {r[0], r[1]};
 }

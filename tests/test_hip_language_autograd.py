@@ -150,3 +150,53 @@ def test_threads_with_streams_of_their_own(binding):
     for th in threads:
         th.join()
     assert not bad, bad
+
+
+def test_a_leaf_of_a_living_eager_graph_is_refused_under_capture():
+    """Only forward passes are captured here: the refusal comes before anything that a backward pass could meet."""
+    from repdl_amd.backend import hip
+    from repdl_amd.nn import functional as F
+
+    if hip.BINDING != "ext":
+        pytest.skip("the compiled binding's check")
+    x, w, b, t = _inputs()
+    calls = {
+        "weight": (w, lambda: F.layer_norm(x, (40,), w, b)),
+        "input": (x, lambda: F.dropout(x, 0.5, (3, 0))),
+        "logits": (None, None),
+    }
+    logits = x.view(2, 3, 40).clone()
+    calls["logits"] = (logits, lambda: F.preference_loss(logits, t)[0])
+    for name, (leaf, call) in calls.items():
+        leaf.requires_grad_()
+        call()  # (the first launch loads the kernels; its graph dies at once)
+        eager = call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = x.detach() + 1  # (something to capture)
+            with pytest.raises(RuntimeError, match=f"{name} still belongs to an eager graph"):
+                call()
+            with torch.no_grad():
+                call()  # (nothing is recorded: no leaf is met)
+        torch.autograd.grad(eager.sum(), leaf)
+        del eager, held
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            again = call().detach()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(again, call().detach())
+        side = torch.cuda.Stream()  # (an eager graph of a side stream stands in nobody's way)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            eager = call()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            again = call().detach()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(again, eager.detach())
+        del eager
+        leaf.requires_grad_(False)
