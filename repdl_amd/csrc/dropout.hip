@@ -111,7 +111,7 @@ int launch_dropout(const void *x, const void *residual, void *y, int64_t n, Drop
 {
     typedef typename LowpType<DT>::T T;
     const int64_t blocks = repdl_cdiv(n, (int64_t)Lowp<DT>::G * DROP_THREADS * DROP_GRANULES);
-    REPDL_REQUIRE(blocks <= REPDL_I32_MAX);
+    REPDL_REQUIRE(blocks <= 0xffffffffLL / DROP_THREADS); // (2^36 elements: more than the memory holds)
     REPDL_LAUNCH((dropout_kernel<DT, RES, STREAM>), dim3((unsigned)blocks), dim3(DROP_THREADS), 0, s, static_cast<const T *>(x),
                  static_cast<const T *>(residual), static_cast<T *>(y), n, d, state, seed, call);
     return repdl_launch_status();

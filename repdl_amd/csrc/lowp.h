@@ -120,5 +120,20 @@ struct Lowp
     }
 };
 
+// A launch counts its threads in 32 bits.  f(first, count) launches workgroups first .. first + count - 1 of `blocks`; rows of a
+// few elements pass that bound long before they fill the memory.
+template <typename F>
+int repdl_launch_slices(int64_t blocks, int threads, F f)
+{
+    const int64_t most = 0xffffffffLL / threads;
+    int rc = REPDL_OK;
+    for (int64_t first = 0; first < blocks && rc == REPDL_OK; first += most)
+    {
+        f(first, (unsigned)(blocks - first < most ? blocks - first : most));
+        rc = repdl_launch_status();
+    }
+    return rc;
+}
+
 static inline bool repdl_known_dtype(int dtype) { return dtype == REPDL_F32 || dtype == REPDL_BF16 || dtype == REPDL_F16; }
 static inline int64_t repdl_dtype_bytes(int dtype) { return dtype == REPDL_F32 ? 4 : 2; }

@@ -776,11 +776,11 @@ template <int PDT>
 __global__ __launch_bounds__(64 * LN_FOLD) void layer_norm_param_kernel(const float *__restrict__ partial,
                                                                         typename LowpType<PDT>::T *__restrict__ gw,
                                                                         typename LowpType<PDT>::T *__restrict__ gb, int64_t N,
-                                                                        int blocks)
+                                                                        int blocks, int64_t first)
 {
     __shared__ float sums[LN_FOLD][64];
     const int lane = threadIdx.x & 63, part = threadIdx.x >> 6;
-    const int64_t col = (int64_t)blockIdx.x * 64 + lane;
+    const int64_t col = (first + blockIdx.x) * 64 + lane;
     float s = 0.0f;
     if (col < 2 * N)
     {
@@ -835,16 +835,19 @@ int launch_layer_norm(const void *x, const void *w, const void *b, void *y, floa
     typedef typename LowpType<DT>::T T;
     typedef typename LowpType<PDT>::T P;
     constexpr int THREADS = TPR < 256 ? 256 : TPR, TEAMS = THREADS / TPR;
-    const dim3 grid((unsigned)repdl_cdiv(M, TEAMS));
-    if (TPR >= 64 && ln_streams<DT>(M, N, y))
-        REPDL_LAUNCH((layer_norm_kernel<DT, PDT, TPR, E, TINY, (TPR >= 64)>), grid, dim3(THREADS), 0, s, static_cast<const T *>(x),
-                     static_cast<const P *>(w), static_cast<const P *>(b), static_cast<T *>(y), mean, rstd, M, (int)N,
-                     (float)(1.0 / (double)N), eps);
-    else
-        REPDL_LAUNCH((layer_norm_kernel<DT, PDT, TPR, E, TINY, false>), grid, dim3(THREADS), 0, s, static_cast<const T *>(x),
-                     static_cast<const P *>(w), static_cast<const P *>(b), static_cast<T *>(y), mean, rstd, M, (int)N,
-                     (float)(1.0 / (double)N), eps);
-    return repdl_launch_status();
+    const bool streams = TPR >= 64 && ln_streams<DT>(M, N, y);
+    return repdl_launch_slices(repdl_cdiv(M, TEAMS), THREADS, [&](int64_t first, unsigned count) {
+        const int64_t row = first * TEAMS;
+        const T *xs = static_cast<const T *>(x) + row * N;
+        T *ys = static_cast<T *>(y) + row * N;
+        float *ms = mean == nullptr ? nullptr : mean + row, *rs = rstd == nullptr ? nullptr : rstd + row;
+        if (streams)
+            REPDL_LAUNCH((layer_norm_kernel<DT, PDT, TPR, E, TINY, (TPR >= 64)>), dim3(count), dim3(THREADS), 0, s, xs,
+                         static_cast<const P *>(w), static_cast<const P *>(b), ys, ms, rs, M - row, (int)N, (float)(1.0 / (double)N), eps);
+        else
+            REPDL_LAUNCH((layer_norm_kernel<DT, PDT, TPR, E, TINY, false>), dim3(count), dim3(THREADS), 0, s, xs,
+                         static_cast<const P *>(w), static_cast<const P *>(b), ys, ms, rs, M - row, (int)N, (float)(1.0 / (double)N), eps);
+    });
 }
 
 template <int DT, int PDT>
@@ -855,10 +858,12 @@ int layer_norm_typed(const void *x, const void *w, const void *b, void *y, float
     {
         typedef typename LowpType<DT>::T T;
         typedef typename LowpType<PDT>::T P;
-        REPDL_LAUNCH((layer_norm_long_kernel<DT, PDT>), dim3((unsigned)M), dim3(1024), 0, s, static_cast<const T *>(x),
-                     static_cast<const P *>(w), static_cast<const P *>(b), static_cast<T *>(y), mean, rstd, M, N,
-                     (float)(1.0 / (double)N), eps);
-        return repdl_launch_status();
+        return repdl_launch_slices(M, 1024, [&](int64_t row, unsigned count) {
+            REPDL_LAUNCH((layer_norm_long_kernel<DT, PDT>), dim3(count), dim3(1024), 0, s, static_cast<const T *>(x) + row * N,
+                         static_cast<const P *>(w), static_cast<const P *>(b), static_cast<T *>(y) + row * N,
+                         mean == nullptr ? nullptr : mean + row, rstd == nullptr ? nullptr : rstd + row, M - row, N,
+                         (float)(1.0 / (double)N), eps);
+        });
     }
     if (N < Lowp<DT>::G)
         return launch_layer_norm<DT, PDT, 4, 16, true>(x, w, b, y, mean, rstd, M, N, eps, s);
@@ -925,10 +930,13 @@ int layer_norm_grad_typed(const void *gy, const void *x, const void *w, const fl
     typedef typename LowpType<PDT>::T P;
     if (N > LN_MAX_ONCHIP)
     {
-        if (gx != nullptr)
-            REPDL_LAUNCH((layer_norm_grad_long_kernel<DT, PDT>), dim3((unsigned)M), dim3(1024), 0, s, static_cast<const T *>(gy),
-                         static_cast<const T *>(x), static_cast<const P *>(w), mean, rstd, static_cast<T *>(gx), N,
-                         (float)(1.0 / (double)N));
+        const int rc = gx == nullptr ? REPDL_OK : repdl_launch_slices(M, 1024, [&](int64_t row, unsigned count) {
+            REPDL_LAUNCH((layer_norm_grad_long_kernel<DT, PDT>), dim3(count), dim3(1024), 0, s, static_cast<const T *>(gy) + row * N,
+                         static_cast<const T *>(x) + row * N, static_cast<const P *>(w), mean + row, rstd + row,
+                         static_cast<T *>(gx) + row * N, N, (float)(1.0 / (double)N));
+        });
+        if (rc != REPDL_OK)
+            return rc;
         if (partial != nullptr)
         {
             const int64_t rpb = ln_rows_per_block(M, N, DT);
@@ -955,9 +963,10 @@ int layer_norm_params(const float *partial, void *gw, void *gb, int64_t M, int64
     typedef typename LowpType<PDT>::T P;
     // (no rows: no blocks, the sums of nothing)
     const int blocks = M == 0 ? 0 : (int)repdl_cdiv(M, ln_rows_per_block(M, N, dtype));
-    REPDL_LAUNCH((layer_norm_param_kernel<PDT>), dim3((unsigned)repdl_cdiv(2 * N, 64)), dim3(64 * LN_FOLD), 0, s, partial,
-                 static_cast<P *>(gw), static_cast<P *>(gb), N, blocks);
-    return repdl_launch_status();
+    return repdl_launch_slices(repdl_cdiv(2 * N, 64), 64 * LN_FOLD, [&](int64_t first, unsigned count) {
+        REPDL_LAUNCH((layer_norm_param_kernel<PDT>), dim3(count), dim3(64 * LN_FOLD), 0, s, partial, static_cast<P *>(gw),
+                     static_cast<P *>(gb), N, blocks, first);
+    });
 }
 
 bool ln_shape_ok(int64_t M, int64_t N, int dtype, int param_dtype)

@@ -40,6 +40,7 @@ struct PrefShape
     int64_t width;  // columns of a chunk
     int64_t ignore; // target of a token that is not counted
     int32_t steps, rows, chunks;
+    uint32_t first; // workgroup of the call that the launch begins with
 };
 
 // Row of logits `row` (0 .. 2 P steps - 1)
@@ -60,9 +61,9 @@ __global__ __launch_bounds__(256) void preference_rows_kernel(const typename Low
     constexpr int G = L::G, GPT = E / G, TEAMS = 256 / TPR;
     __shared__ float wave_m[4], wave_s[4];
     const int tid = threadIdx.x, j = tid % TPR;
-    if (blockIdx.x == 0 && tid == 0)
+    if (p.first + blockIdx.x == 0 && tid == 0)
         *counter = 0; // (of the pairs kernel, which the stream orders after this one)
-    const uint32_t item = __builtin_amdgcn_readfirstlane(blockIdx.x * TEAMS + tid / TPR); // (row, chunk): the wave's
+    const uint32_t item = __builtin_amdgcn_readfirstlane((p.first + blockIdx.x) * TEAMS + tid / TPR); // (row, chunk): the wave's
     const uint32_t row = TPR == 64 ? item : item / (uint32_t)p.chunks;
     const uint32_t chunk = TPR == 64 ? 0 : item - row * (uint32_t)p.chunks;
     if (row >= (uint32_t)p.rows)
@@ -210,7 +211,7 @@ __global__ __launch_bounds__(PAIR_THREADS) void preference_pairs_kernel(const in
     __shared__ double scratch[PAIR_THREADS / 64];
     __shared__ int last;
     __shared__ PairTables tables;
-    const int tid = threadIdx.x, pair = blockIdx.x;
+    const int tid = threadIdx.x, pair = (int)(p.first + blockIdx.x);
     // the first half of the workgroup takes the preferred answer's tokens, the second half the other's
     constexpr int HALF = PAIR_THREADS / 2;
     const int side = tid / HALF;
@@ -323,7 +324,7 @@ __global__ __launch_bounds__(256, 4) void preference_grad_kernel(const typename 
     typedef Lowp<DT> L;
     constexpr int G = L::G, GPT = E / G, TEAMS = 256 / TPR;
     const int tid = threadIdx.x, j = tid % TPR;
-    const uint32_t item = __builtin_amdgcn_readfirstlane(blockIdx.x * TEAMS + tid / TPR);
+    const uint32_t item = __builtin_amdgcn_readfirstlane((p.first + blockIdx.x) * TEAMS + tid / TPR);
     const uint32_t row = TPR == 64 ? item : item / (uint32_t)p.chunks;
     const uint32_t chunk = TPR == 64 ? 0 : item - row * (uint32_t)p.chunks;
     if (row >= (uint32_t)p.rows)
@@ -423,6 +424,7 @@ PrefShape pref_shape(int64_t pairs, int64_t steps, int64_t vocab, int64_t seq_st
     p.ignore = ignore;
     p.steps = (int32_t)steps;
     p.rows = (int32_t)(2 * pairs * steps);
+    p.first = 0;
     pref_chunks(vocab, most, p.chunks, p.width);
     return p;
 }
@@ -434,42 +436,48 @@ bool pref_streams(const PrefShape &p)
 }
 
 template <int DT>
-int launch_pref_rows(const void *logits, const int64_t *target, float2 *part, float *picked, int *counter, const PrefShape &p, hipStream_t s)
+int launch_pref_rows(const void *logits, const int64_t *target, float2 *part, float *picked, int *counter, PrefShape p, hipStream_t s)
 {
     const auto *x = static_cast<const typename LowpType<DT>::T *>(logits);
+    const bool by_wave = p.vocab <= PREF_WAVE, streams = pref_streams<DT>(p);
     // (one workgroup at least: it clears the counter)
-    const unsigned by_wave = (unsigned)(p.rows == 0 ? 1 : repdl_cdiv(p.rows, 4));
-    const unsigned by_chunk = (unsigned)(p.rows == 0 ? 1 : (int64_t)p.rows * p.chunks);
-    if (p.vocab <= PREF_WAVE_SMALL)
-        REPDL_LAUNCH((preference_rows_kernel<DT, 64, PREF_SMALL_E, false>), dim3(by_wave), dim3(256), 0, s, x, target, part, picked, counter, p);
-    else if (p.vocab <= PREF_WAVE)
-        REPDL_LAUNCH((preference_rows_kernel<DT, 64, PREF_E, false>), dim3(by_wave), dim3(256), 0, s, x, target, part, picked, counter, p);
-    else if (pref_streams<DT>(p))
-        REPDL_LAUNCH((preference_rows_kernel<DT, 256, PREF_E, true>), dim3(by_chunk), dim3(256), 0, s, x, target, part, picked, counter, p);
-    else
-        REPDL_LAUNCH((preference_rows_kernel<DT, 256, PREF_E, false>), dim3(by_chunk), dim3(256), 0, s, x, target, part, picked, counter, p);
-    return repdl_launch_status();
+    const int64_t blocks = p.rows == 0 ? 1 : by_wave ? repdl_cdiv(p.rows, 4) : (int64_t)p.rows * p.chunks;
+    return repdl_launch_slices(blocks, 256, [&](int64_t first, unsigned count) {
+        p.first = (uint32_t)first;
+        if (p.vocab <= PREF_WAVE_SMALL)
+            REPDL_LAUNCH((preference_rows_kernel<DT, 64, PREF_SMALL_E, false>), dim3(count), dim3(256), 0, s, x, target, part, picked, counter, p);
+        else if (by_wave)
+            REPDL_LAUNCH((preference_rows_kernel<DT, 64, PREF_E, false>), dim3(count), dim3(256), 0, s, x, target, part, picked, counter, p);
+        else if (streams)
+            REPDL_LAUNCH((preference_rows_kernel<DT, 256, PREF_E, true>), dim3(count), dim3(256), 0, s, x, target, part, picked, counter, p);
+        else
+            REPDL_LAUNCH((preference_rows_kernel<DT, 256, PREF_E, false>), dim3(count), dim3(256), 0, s, x, target, part, picked, counter, p);
+    });
 }
 
 constexpr int PREF_GRAD_E = 32;
 
 template <int DT>
 int launch_pref_grad(const void *logits, const int64_t *target, const float2 *row_stats, const float *coef, const float *grad_loss,
-                     void *grad_logits, const PrefShape &p, hipStream_t s)
+                     void *grad_logits, PrefShape p, hipStream_t s)
 {
     typedef typename LowpType<DT>::T T;
     const T *x = static_cast<const T *>(logits);
     T *gx = static_cast<T *>(grad_logits);
-    if (p.vocab <= PREF_WAVE_SMALL)
-        REPDL_LAUNCH((preference_grad_kernel<DT, 64, PREF_SMALL_E, false>), dim3((unsigned)repdl_cdiv(p.rows, 4)), dim3(256), 0, s, x, target,
-                     row_stats, coef, grad_loss, gx, p);
-    else if (pref_streams<DT>(p) && p.vocab % Lowp<DT>::G == 0 && (reinterpret_cast<uintptr_t>(gx) & 15) == 0)
-        REPDL_LAUNCH((preference_grad_kernel<DT, 256, PREF_GRAD_E, true>), dim3((unsigned)((int64_t)p.rows * p.chunks)), dim3(256), 0, s, x,
-                     target, row_stats, coef, grad_loss, gx, p);
-    else
-        REPDL_LAUNCH((preference_grad_kernel<DT, 256, PREF_GRAD_E, false>), dim3((unsigned)((int64_t)p.rows * p.chunks)), dim3(256), 0, s, x,
-                     target, row_stats, coef, grad_loss, gx, p);
-    return repdl_launch_status();
+    const bool by_wave = p.vocab <= PREF_WAVE_SMALL;
+    const bool streams = pref_streams<DT>(p) && p.vocab % Lowp<DT>::G == 0 && (reinterpret_cast<uintptr_t>(gx) & 15) == 0;
+    return repdl_launch_slices(by_wave ? repdl_cdiv(p.rows, 4) : (int64_t)p.rows * p.chunks, 256, [&](int64_t first, unsigned count) {
+        p.first = (uint32_t)first;
+        if (by_wave)
+            REPDL_LAUNCH((preference_grad_kernel<DT, 64, PREF_SMALL_E, false>), dim3(count), dim3(256), 0, s, x, target, row_stats, coef,
+                         grad_loss, gx, p);
+        else if (streams)
+            REPDL_LAUNCH((preference_grad_kernel<DT, 256, PREF_GRAD_E, true>), dim3(count), dim3(256), 0, s, x, target, row_stats, coef,
+                         grad_loss, gx, p);
+        else
+            REPDL_LAUNCH((preference_grad_kernel<DT, 256, PREF_GRAD_E, false>), dim3(count), dim3(256), 0, s, x, target, row_stats, coef,
+                         grad_loss, gx, p);
+    });
 }
 } // namespace
 
@@ -481,7 +489,7 @@ REPDL_API int repdl_hip_preference_loss(const void *logits, const int64_t *targe
     REPDL_REQUIRE(pref_shape_ok(pairs, steps, vocab, seq_stride, step_stride, dtype));
     REPDL_REQUIRE(loss != nullptr && logps != nullptr && (steps == 0 || (logits != nullptr && target != nullptr)));
     hipStream_t s = repdl_stream(stream);
-    const PrefShape p = pref_shape(pairs, steps, vocab, seq_stride, step_stride, ignore_index, PREF_CHUNK);
+    PrefShape p = pref_shape(pairs, steps, vocab, seq_stride, step_stride, ignore_index, PREF_CHUNK);
     // scratch: (m, sum) per row and chunk, the pairs' losses, the target's logit per row, a counter
     const size_t parts = (size_t)p.rows * (size_t)p.chunks;
     char *work = nullptr;
@@ -497,11 +505,11 @@ REPDL_API int repdl_hip_preference_loss(const void *logits, const int64_t *targe
              : dtype == REPDL_BF16 ? launch_pref_rows<REPDL_BF16>(logits, target, part, picked, counter, p, s)
                                    : launch_pref_rows<REPDL_F16>(logits, target, part, picked, counter, p, s);
     if (rc == REPDL_OK)
-    {
-        REPDL_LAUNCH(preference_pairs_kernel, dim3((unsigned)pairs), dim3(PAIR_THREADS), 0, s, target, part, picked, ref_logps, pair_loss,
-                     counter, loss, logps, reinterpret_cast<float2 *>(row_stats), coef, p, (int)pairs, beta, label_smoothing);
-        rc = repdl_launch_status();
-    }
+        rc = repdl_launch_slices(pairs, PAIR_THREADS, [&](int64_t first, unsigned count) { // (the counter goes on from slice to slice)
+            p.first = (uint32_t)first;
+            REPDL_LAUNCH(preference_pairs_kernel, dim3(count), dim3(PAIR_THREADS), 0, s, target, part, picked, ref_logps, pair_loss,
+                         counter, loss, logps, reinterpret_cast<float2 *>(row_stats), coef, p, (int)pairs, beta, label_smoothing);
+        });
     e = repdl_ws_release(work, s);
     return rc != REPDL_OK ? rc : (int)e;
 }

@@ -354,6 +354,30 @@ def test_side_stream_and_graph():
         assert all(torch.equal(p, q) for p, q in zip(got, step()))
 
 
+def test_more_threads_than_a_launch_counts():
+    """A launch counts its threads in 32 bits: 2^30 rows of four threads, and 2 x 2^27 columns of sixteen, pass that; the rows (columns)
+    behind the bound have the bits of those before it."""
+    from repdl_amd.nn import functional as F
+
+    rows = gen.normal_like(70, 1 << 18, 2).to(torch.bfloat16).cuda()
+    w, b = gen.normal_like(71, 2).cuda(), gen.normal_like(72, 2).cuda()
+
+    def both(x):
+        x = x.requires_grad_()
+        y = F.layer_norm(x, (2,), w, b)
+        return y.detach(), torch.autograd.grad(y, x, x.detach())[0]
+
+    want = both(rows.clone())
+    for got, part in zip(both(rows.repeat(4096 + 1, 1)), want):  # (2^30 + 2^18 rows)
+        assert (got.view(4096 + 1, -1) == part.view(-1)).all()
+    del got
+    cols = gen.normal_like(73, 2, 1 << 20).to(torch.bfloat16).cuda()
+    x, gy = (c.repeat(129).view(1, -1) for c in cols)
+    w, b = (torch.ones(x.shape[1], dtype=torch.bfloat16, device="cuda", requires_grad=True) for _ in range(2))
+    gw, gb = torch.autograd.grad(F.layer_norm(x, x.shape[1:], w, b), (w, b), gy)
+    assert torch.equal(gb, gy[0]) and gw.any() and (gw.view(129, -1) == gw[:1 << 20]).all()
+
+
 def test_both_bindings():
     from repdl_amd.backend import hip_ctypes
 

@@ -136,6 +136,56 @@ def test_bits_of_the_documented_order(case, kind, model):
     assert torch.equal(got[1].cpu(), want[1]) and torch.equal(got[0].cpu(), want[0])
 
 
+# A launch counts its threads in 32 bits; what lies behind that bound has the bits of what lies before it.
+def test_more_pairs_than_a_launch_counts():
+    from repdl_amd import ops
+
+    x, t, ref = data(1021, 1, 5, "f32", seed=50)
+    small = ops.preference_loss(x, t, ref)
+    times = 4109  # (4195289 pairs of 1024 threads)
+    wide = [v.view(2, 1021, -1).repeat(1, times, 1).view(2 * 1021 * times, *v.shape[1:]) for v in (x, t, ref)]
+    loss, logps, stats, coef = ops.preference_loss(*wide)
+    assert (logps.view(2, times, 1021) == small[1].view(2, 1, 1021)).all()
+    assert (stats.view(2, times, 1021, 2) == small[2].view(2, 1, 1021, 2)).all()
+    # (the sum adds 4097 + 15 + 6 binary64 roundings; the result rounds once, the other's did too: two half steps.  Coefficients alike.)
+    assert abs(float(loss) - float(small[0])) <= 2 * (U + 4200 * 2.0 ** -53) * float(small[0])
+    assert ((coef.view(2, times, 1021).double() * times - small[3].view(2, 1, 1021).double()).abs() <= 2.001 * U * small[3].view(2, 1, 1021).double().abs()).all()
+
+
+def test_more_rows_than_a_launch_counts():
+    from repdl_amd import ops
+
+    P, steps = 8, 4194310  # (67108960 rows, 64 threads each)
+    x = (gen.normal_like(51, 2 * P, 1000, 3) * 3).to(torch.bfloat16).cuda().repeat(1, 4195, 1)[:, :steps]
+    t = gen.labels(52, 2 * P * 1000, 3).view(2 * P, 1000).cuda().repeat(1, 4195)[:, :steps].contiguous()
+    loss, logps, stats, coef = ops.preference_loss(x, t, None)
+    g = torch.ones((), device="cuda")
+    gx = ops.preference_loss_grad(x, t, stats, coef, g)
+    few = [0, 7, 8, 15]  # the first and the last pair
+    alone = ops.preference_loss(x[few], t[few], None)
+    assert torch.equal(logps[few], alone[1]) and torch.equal(stats[few], alone[2])
+    assert torch.equal(gx[few], ops.preference_loss_grad(x[few], t[few], stats[few], coef[few], g))
+    # (over millions of tokens a pair's margin leaves a coefficient of one side or of zero: coefficients of our own show every row)
+    coef = torch.linspace(-1.0, 1.0, 2 * P, device="cuda")
+    gx = ops.preference_loss_grad(x, t, stats, coef, g)
+    assert torch.equal(gx[few], ops.preference_loss_grad(x[few], t[few], stats[few], coef[few], g)) and gx[15, -50:].any()
+
+
+def test_more_chunks_than_a_launch_counts():
+    """One row of logits, seen 16777400 times, 256 threads each."""
+    from repdl_amd import ops
+
+    steps, g = 8388700, torch.ones((), device="cuda")
+    row = (gen.normal_like(53, 1, 1, 4097) * 3).half().cuda()
+    t = torch.full((2, steps), 1001, device="cuda")
+    stats = ops.preference_loss(row.expand(2, steps, 4097), t, None)[2]
+    assert (stats == ops.preference_loss(row.expand(2, 1, 4097), t[:, :1], None)[2]).all()
+    row, coef = row[:, :, :1025], torch.tensor([1.0, -1.0], device="cuda")  # (34 GB of gradients)
+    gx = ops.preference_loss_grad(row.expand(2, steps, 1025), t, stats, coef, g)
+    want = ops.preference_loss_grad(row.expand(2, 1, 1025), t[:, :1], stats[:, :1], coef, g)
+    assert want.any() and (gx[0, :500] == want[0]).all() and (gx[1, :500] == want[1]).all() and (gx[1, -500:] == want[1]).all()
+
+
 def test_incoming_gradient_scales():
     from repdl_amd.nn import functional as F
 
