@@ -307,15 +307,18 @@ int repdl_hip_bn_gweight_term(const float *x, const float *mean, const float *st
  * dtype or REPDL_F32; mean and rstd are [M] binary32, for the backward pass (both NULL: not wanted).  Per row:
  *   mean = S(x_j) * float(1/N),  var = S(RN(d_j * d_j)) * float(1/N) with d_j = RN(x_j - mean),
  *   rstd = RN(1 / RN(sqrt(RN(var + eps)))),  y_j = RN(RN(RN(d_j * rstd) * weight_j) + bias_j)
+ * A row far above its spread, RN(mean * mean) > RN(256 * var), is centred in two numbers:
+ *   better = RN(mean + RN(S(d_j) * float(1/N))),  e_j = RN(d_j - (better - mean)),  rest = S(e_j) * float(1/N),  d_j = RN(e_j - rest),
+ * var from these d_j, and `better` is its mean; a constant row is its bias.
  * S is a binary32 sum whose order N and the type determine alone: the same row gives the same bits whatever the other
  * rows, the addresses, the stream and the device.
- * Backward, with xh_j = RN(d_j * rstd) and g_j = RN(grad_y_j * weight_j):
+ * Backward, with d_j = RN(x_j - mean) (where RN(|mean| * rstd) > 16: RN(RN(x_j - mean) - rest)), xh_j = RN(d_j * rstd) and g_j = RN(grad_y_j * weight_j):
  *   grad_x_j    = RN(rstd * RN(RN(g_j - c1) - RN(xh_j * c2))),  c1 = S(g_j) * float(1/N),  c2 = S(RN(g_j * xh_j)) * float(1/N)
  *   grad_weight = S over the rows of RN(grad_y_ij * xh_ij),  grad_bias = S over the rows of grad_y_ij
  * (the order of the sums over rows is a function of M, N and the type; they are rounded to param_dtype at the end).  Any of
  * grad_x, grad_weight, grad_bias may be NULL: not wanted.  M = 0 gives zeros in grad_weight and grad_bias.
- * Scratch (see "Scratch memory"): at most 512 rows of 2 N floats for the two sums over rows, where they are wanted; none for at
- * most 256 rows of at most 16384 elements. */
+ * Scratch (see "Scratch memory"): at most 512 rows of 2 N floats for the two sums over rows, where they are wanted, and a float
+ * per row of more than 16384 elements; none for at most 256 rows of at most 16384 elements. */
 int repdl_hip_layer_norm(const void *x, const void *weight, const void *bias, void *y, float *mean, float *rstd, int64_t M,
                          int64_t N, float eps, int dtype, int param_dtype, void *stream);
 int repdl_hip_layer_norm_grad(const void *grad_y, const void *x, const void *weight, const float *mean, const float *rstd,

@@ -5,6 +5,14 @@
 //   g_j = gy_j w_j,  gx_j = rstd ((g_j - mean(g)) - xh_j mean(g xh))
 //   gw_j = sum_i gy_ij xh_ij,  gb_j = sum_i gy_ij
 //
+// Offset rows.  A binary32 mean is off by a few roundings of the row's level: harmless where the level is near the spread, ruin where
+// it is a thousand times above it (a constant row came out as y = -1 instead of 0).  A row with |mean| > 16 spreads is therefore centred in
+// two numbers: the mean corrected by S(x_j - mean) / N, then rest = S(x_j - mean) / N, and x_j - mean - rest stands for the centred
+// x_j.  The backward pass has the corrected mean and makes `rest` again.  Such a row costs two more sums over its registers and the squares
+// again forward, one sum backward; any other (off by at most 17 spreads' worth of its sum's roundings) a comparison.  No row / every row offset:
+// 8192 x 1024 f32 forward 0.0124 / 0.0129 ms, backward 0.0219 / 0.0221; 8192 x 4096 bf16 0.0243 / 0.0276, 0.0421 / 0.0434; 32768 x 2056 f16 0.0536 /
+// 0.0648, 0.092 / 0.094.  (Sixteen: at that level the mean's error is what a row of no offset has in a sum of its length anyway.)
+//
 // Every operation above is one IEEE binary32 operation (nothing is fused; the square root and the reciprocal are the
 // correctly rounded ones of crmath.h; "(1/N)" is one multiplication by float(1/N), as in the library's averages), so a
 // result is a function of the inputs and of the order of the sums alone.  That order is fixed by the row length, the type
@@ -35,6 +43,7 @@ __host__ __device__ constexpr int ln_threads_per_row(int64_t N, int E)
     return t;
 }
 constexpr int ln_grad_threads(int tpr) { return tpr < 256 ? 256 : tpr; }
+constexpr int64_t LN_FEW_ROWS = 256; // (up to here one launch makes all gradients, see ln_few_rows)
 constexpr int64_t LN_MAX_ONCHIP = 16384; // (1024 threads of 16 elements; longer rows are read from memory for every pass)
 
 // Elements per thread: 16, or 24 in a 16-bit type whose row would leave many of 16 elements' threads without any (half the threads
@@ -110,6 +119,19 @@ __device__ __forceinline__ float granule_sum(const float *v)
 }
 
 __device__ __forceinline__ float ln_rstd(float var, float eps) { return crm_div(1.0f, crm_sqrt(var + eps)); }
+
+// An offset row (see the top), from what the forward pass has and from what the backward pass has.
+constexpr float LN_OFFSET = 16.0f;
+__device__ __forceinline__ bool ln_offset(float mean, float var) { return mean * mean > LN_OFFSET * LN_OFFSET * var; }
+__device__ __forceinline__ bool ln_offset_saved(float mean, float rstd) { return __builtin_fabsf(mean) * rstd > LN_OFFSET; }
+
+// Does any of the rows that have to go through a row sum together have `offset` set: those of a wave, and where a row's
+// threads are two of a workgroup's four waves (their sums meet at a barrier) those of the workgroup: `other` says so of the other row.
+template <int TPR>
+__device__ __forceinline__ bool ln_any(bool offset, bool other)
+{
+    return TPR <= 64 ? __any(offset) : TPR == 128 ? offset || other : offset;
+}
 
 // Parameters are read in granules of the activation's element count, whatever their own type.
 template <int G, int PDT>
@@ -214,7 +236,7 @@ struct RowGranules
 };
 
 template <int DT, int PDT, int TPR, int E, bool TINY, bool STREAM>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_kernel(
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR, 8) void layer_norm_kernel(
     const typename LowpType<DT>::T *__restrict__ x, const typename LowpType<PDT>::T *__restrict__ w,
     const typename LowpType<PDT>::T *__restrict__ b, typename LowpType<DT>::T *__restrict__ y, float *__restrict__ mean_out,
     float *__restrict__ rstd_out, int64_t M, int N, float inv_n, float eps)
@@ -223,6 +245,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_kernel(
     constexpr int G = L::G, GPT = E / G;
     constexpr int THREADS = TPR < 256 ? 256 : TPR, TEAMS = THREADS / TPR;
     __shared__ float scratch[2][TEAMS][TPR / 64 + 1];
+    __shared__ int offsets[TEAMS];
     const int tid = threadIdx.x, team = tid / TPR, j = tid % TPR;
     const int64_t row = wave_value<TPR>((int64_t)blockIdx.x * TEAMS + team);
     const bool live = row < M;
@@ -242,21 +265,57 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void layer_norm_kernel(
         s[0] = s[0] + rg.sum(v[i], i, N);
     }
     team_sum<TPR, 1>(s, scratch[0][team], j);
-    const float mean = s[0] * inv_n;
-    float q[1] = {0.0f};
+    float mean = s[0] * inv_n;
+    // v - by, squared and summed: by the mean, then (in an offset row) by what the mean leaves
+    float q[1];
+    auto centre = [&](float by) {
+        q[0] = 0.0f;
 #pragma unroll
-    for (int i = 0; i < GPT; i++)
-    {
-        float sq[G];
-#pragma unroll
-        for (int k = 0; k < G; k++)
+        for (int i = 0; i < GPT; i++)
         {
-            v[i][k] = v[i][k] - mean;
-            sq[k] = v[i][k] * v[i][k];
+            float sq[G];
+#pragma unroll
+            for (int k = 0; k < G; k++)
+            {
+                v[i][k] = v[i][k] - by;
+                sq[k] = v[i][k] * v[i][k];
+            }
+            q[0] = q[0] + rg.sum(sq, i, N);
         }
-        q[0] = q[0] + rg.sum(sq, i, N);
-    }
+    };
+    centre(mean);
     team_sum<TPR, 1>(q, scratch[1][team], j);
+    const bool offset = ln_offset(mean, q[0] * inv_n);
+    bool other = false;
+    if (TPR == 128)
+    {
+        if (j == 0)
+            offsets[team] = offset;
+        lds_barrier();
+        other = offsets[TEAMS - 1 - team];
+    }
+    if (ln_any<TPR>(offset, other)) // (a row that is not offset but goes along ends with the bits it had)
+    {
+        s[0] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < GPT; i++)
+            s[0] = s[0] + rg.sum(v[i], i, N);
+        team_sum<TPR, 1>(s, scratch[0][team], j);
+        const float better = mean + s[0] * inv_n, by = offset ? better - mean : 0.0f; // (exact)
+        mean = offset ? better : mean;
+        s[0] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < GPT; i++)
+        {
+#pragma unroll
+            for (int k = 0; k < G; k++)
+                v[i][k] = v[i][k] - by;
+            s[0] = s[0] + rg.sum(v[i], i, N);
+        }
+        team_sum<TPR, 1>(s, scratch[1][team], j);
+        centre(offset ? s[0] * inv_n : 0.0f);
+        team_sum<TPR, 1>(q, scratch[0][team], j);
+    }
     const float rstd = ln_rstd(q[0] * inv_n, eps);
     if (!live)
         return;
@@ -316,23 +375,40 @@ __global__ __launch_bounds__(1024) void layer_norm_long_kernel(
     }
     team_sum<TPR, 1>(s, scratch[0], j);
     const float mean = s[0] * inv_n;
-    float q[1] = {0.0f};
-    for (int64_t c = (int64_t)j * G; c < N; c += TPR * G)
-    {
-        L::load(xr, c, N, mean, v);
-#pragma unroll
-        for (int k = 0; k < G; k++)
+    float better = 0.0f, rest = 0.0f; // of an offset row
+    // S(x_j - mean - better - rest), or of its square
+    auto centred = [&](bool square) {
+        float t = 0.0f;
+        for (int64_t c = (int64_t)j * G; c < N; c += TPR * G)
         {
-            v[k] = c + k < N ? v[k] - mean : 0.0f;
-            v[k] = v[k] * v[k];
+            L::load(xr, c, N, mean, v);
+#pragma unroll
+            for (int k = 0; k < G; k++)
+            {
+                v[k] = c + k < N ? ((v[k] - mean) - better) - rest : 0.0f;
+                v[k] = square ? v[k] * v[k] : v[k];
+            }
+            t = t + granule_sum<G>(v);
         }
-        q[0] = q[0] + granule_sum<G>(v);
-    }
+        return t;
+    };
+    float q[1] = {centred(true)};
     team_sum<TPR, 1>(q, scratch[1], j);
+    if (ln_offset(mean, q[0] * inv_n)) // (the whole workgroup's)
+    {
+        s[0] = centred(false);
+        team_sum<TPR, 1>(s, scratch[0], j);
+        better = (mean + s[0] * inv_n) - mean; // (exact)
+        s[0] = centred(false);
+        team_sum<TPR, 1>(s, scratch[1], j);
+        rest = s[0] * inv_n;
+        q[0] = centred(true);
+        team_sum<TPR, 1>(q, scratch[0], j);
+    }
     const float rstd = ln_rstd(q[0] * inv_n, eps);
     if (mean_out != nullptr && j == 0)
     {
-        mean_out[row] = mean;
+        mean_out[row] = mean + better;
         rstd_out[row] = rstd;
     }
     typename L::T *yr = y + row * N;
@@ -345,7 +421,7 @@ __global__ __launch_bounds__(1024) void layer_norm_long_kernel(
 #pragma unroll
         for (int k = 0; k < G; k++)
         {
-            v[k] = (v[k] - mean) * rstd;
+            v[k] = (((v[k] - mean) - better) - rest) * rstd;
             if (w != nullptr)
                 v[k] = v[k] * wv[k];
             if (b != nullptr)
@@ -356,6 +432,23 @@ __global__ __launch_bounds__(1024) void layer_norm_long_kernel(
 }
 
 // ---- backward ---------------------------------------------------------------------------------
+// An offset row's centred values once more (those of a row that goes along stay as they are).
+template <int TPR, typename Granules, int GPT, int G>
+__device__ __forceinline__ void ln_centre_again(const Granules &rg, float (&xv)[GPT][G], bool offset, float *scratch, int j, int N, float inv_n)
+{
+    float t[1] = {0.0f};
+#pragma unroll
+    for (int i = 0; i < GPT; i++)
+        t[0] = t[0] + rg.sum(xv[i], i, N);
+    team_sum<TPR, 1>(t, scratch, j);
+    const float rest = offset ? t[0] * inv_n : 0.0f;
+#pragma unroll
+    for (int i = 0; i < GPT; i++)
+#pragma unroll
+        for (int k = 0; k < G; k++)
+            xv[i][k] = xv[i][k] - rest;
+}
+
 // A workgroup owns a run of consecutive rows, its teams taking them in turn; a thread meets the same columns in every row and
 // adds up their gw and gb in registers.  At the end the teams' sums are added in order through LDS and written as one row of
 // `partial` [blocks][2][N]; layer_norm_param_kernel adds the blocks.  x and gy are read once, gx is written once.
@@ -374,6 +467,7 @@ __global__ __launch_bounds__(ln_grad_threads(TPR), TPR < 1024 ? 2 : 4) void laye
     constexpr int THREADS = ln_grad_threads(TPR), TEAMS = THREADS / TPR;
     __shared__ float scratch[2][TEAMS][2 * (TPR / 64) + 1];
     __shared__ float fold[TEAMS > 1 ? THREADS * E : 1];
+    __shared__ int some;
     const int tid = threadIdx.x, team = tid / TPR, j = tid % TPR;
     const int64_t r0 = (int64_t)blockIdx.x * rows_per_block;
     const int64_t r1 = r0 + rows_per_block < M ? r0 + rows_per_block : M;
@@ -409,6 +503,20 @@ __global__ __launch_bounds__(ln_grad_threads(TPR), TPR < 1024 ? 2 : 4) void laye
         next_rstd = rstd_in[rr];
     };
     fetch(r0 + team);
+    bool other = false;
+    if (TPR == 128) // (any row of the run, asked once: asking for the other team's row at every step took 100 ns a step)
+    {
+        bool found = false;
+        for (int64_t r = r0 + tid; r < r1; r += THREADS)
+            found = found || ln_offset_saved(mean_in[r], rstd_in[r]);
+        if (tid == 0)
+            some = 0;
+        lds_barrier();
+        if (found)
+            some = 1;
+        lds_barrier();
+        other = some;
+    }
     int half = 0;
     for (int64_t base = r0; base < r1; base += TEAMS)
     {
@@ -422,8 +530,19 @@ __global__ __launch_bounds__(ln_grad_threads(TPR), TPR < 1024 ? 2 : 4) void laye
             L::unpack(ng[i], gv[i]);
         }
         const float mean = next_mean, rstd = next_rstd;
+        const bool offset = ln_offset_saved(mean, rstd), any = ln_any<TPR>(offset, other);
         if (base + TEAMS < r1)
             fetch(row + TEAMS);
+#pragma unroll
+        for (int i = 0; i < GPT; i++)
+#pragma unroll
+            for (int k = 0; k < G; k++)
+                xv[i][k] = xv[i][k] - mean;
+        if (any)
+        {
+            ln_centre_again<TPR>(rg, xv, offset, scratch[half][team], j, N, inv_n);
+            half ^= 1;
+        }
         float s[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < GPT; i++)
@@ -431,7 +550,7 @@ __global__ __launch_bounds__(ln_grad_threads(TPR), TPR < 1024 ? 2 : 4) void laye
             float p[G];
 #pragma unroll
             for (int k = 0; k < G; k++)
-                xv[i][k] = (xv[i][k] - mean) * rstd;
+                xv[i][k] = xv[i][k] * rstd;
             if (live && partial != nullptr)
             {
 #pragma unroll
@@ -531,9 +650,10 @@ __global__ __launch_bounds__(ln_grad_threads(TPR), TPR < 1024 ? 2 : 4) void laye
 // Few rows: one launch for all three gradients.  The first `row_blocks` workgroups make gx, a row per team; the others make gw and gb
 // straight from x, gy and the rows' statistics, 16 granules of columns a workgroup, every 16 threads taking every
 // (threads / 16)-th row in turn and their sums added in order through LDS.  x and gy are read twice, the second time out of
-// the caches, and there are no partial sums, no second launch and no scratch.
+// the caches, and there are no partial sums, no second launch and no scratch.  Where rows are offset, each of these workgroups sums them
+// all for itself (every row: 64 x 1024 f32 0.018 ms instead of 0.003, 256 x 16384 f32 0.153 instead of 0.014).
 template <int DT, int PDT, int TPR, int E, bool TINY>
-__global__ __launch_bounds__(ln_grad_threads(TPR)) void layer_norm_grad_few_kernel(
+__global__ __launch_bounds__(ln_grad_threads(TPR), TPR == 1024 && DT == REPDL_F32 ? 8 : 1) void layer_norm_grad_few_kernel(
     const typename LowpType<DT>::T *__restrict__ gy, const typename LowpType<DT>::T *__restrict__ x,
     const typename LowpType<PDT>::T *__restrict__ w, const float *__restrict__ mean_in, const float *__restrict__ rstd_in,
     typename LowpType<DT>::T *__restrict__ gx, typename LowpType<PDT>::T *__restrict__ gw, typename LowpType<PDT>::T *__restrict__ gb,
@@ -542,12 +662,13 @@ __global__ __launch_bounds__(ln_grad_threads(TPR)) void layer_norm_grad_few_kern
     typedef Lowp<DT> L;
     constexpr int G = L::G, GPT = E / G;
     constexpr int THREADS = ln_grad_threads(TPR), TEAMS = THREADS / TPR, GROUPS = THREADS / 16;
-    __shared__ float scratch[TEAMS][2 * (TPR / 64) + 1];
+    __shared__ float scratch[2][TEAMS][2 * (TPR / 64) + 1];
     __shared__ float fold[GROUPS][16 * G];
-    const int tid = threadIdx.x;
+    __shared__ float rest[LN_FEW_ROWS];
+    __shared__ int some;
+    const int tid = threadIdx.x, team = tid / TPR, j = tid % TPR;
     if ((int)blockIdx.x < row_blocks)
     {
-        const int team = tid / TPR, j = tid % TPR;
         const int64_t row = wave_value<TPR>((int64_t)blockIdx.x * TEAMS + team);
         const bool live = row < M;
         const int64_t rr = live ? row : M - 1;
@@ -560,14 +681,30 @@ __global__ __launch_bounds__(ln_grad_threads(TPR)) void layer_norm_grad_few_kern
             rgy[i] = rg.template load<false>(gy + rr * N, i, N);
         }
         const float mean = mean_in[rr], rstd = rstd_in[rr];
+        const bool offset = ln_offset_saved(mean, rstd);
+        bool other = false;
+        if (TPR == 128)
+        {
+            const int64_t ro = wave_value<TPR>(row + 1 - 2 * team < M ? row + 1 - 2 * team : M - 1);
+            other = ln_offset_saved(mean_in[ro], rstd_in[ro]);
+        }
         float xv[GPT][G], gv[GPT][G];
+#pragma unroll
+        for (int i = 0; i < GPT; i++)
+        {
+            L::unpack(rx[i], xv[i]);
+            L::unpack(rgy[i], gv[i]);
+#pragma unroll
+            for (int k = 0; k < G; k++)
+                xv[i][k] = xv[i][k] - mean;
+        }
+        if (ln_any<TPR>(offset, other))
+            ln_centre_again<TPR>(rg, xv, offset, scratch[1][team], j, N, inv_n);
         float s[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < GPT; i++)
         {
             float p[G];
-            L::unpack(rx[i], xv[i]);
-            L::unpack(rgy[i], gv[i]);
             if (w != nullptr)
             {
                 rg.template param<PDT>(w, i, N, p);
@@ -578,13 +715,13 @@ __global__ __launch_bounds__(ln_grad_threads(TPR)) void layer_norm_grad_few_kern
 #pragma unroll
             for (int k = 0; k < G; k++)
             {
-                xv[i][k] = (xv[i][k] - mean) * rstd;
+                xv[i][k] = xv[i][k] * rstd;
                 p[k] = gv[i][k] * xv[i][k];
             }
             s[0] = s[0] + rg.sum(gv[i], i, N);
             s[1] = s[1] + rg.sum(p, i, N);
         }
-        team_sum<TPR, 2>(s, scratch[team], j);
+        team_sum<TPR, 2>(s, scratch[0][team], j);
         const float m1 = s[0] * inv_n, m2 = s[1] * inv_n;
         if (live)
         {
@@ -606,51 +743,112 @@ __global__ __launch_bounds__(ln_grad_threads(TPR)) void layer_norm_grad_few_kern
     const int wanted = (((int)blockIdx.x - row_blocks) * 16 + lane) * G;
     const int c = TINY ? 0 : (wanted < N - G ? wanted : N - G);
     float aw[G], ab[G];
+    bool found = false;
+    auto accumulate = [&](auto with_rest) {
+        constexpr bool REST = decltype(with_rest)::value;
 #pragma unroll
-    for (int k = 0; k < G; k++)
-        aw[k] = ab[k] = 0.0f;
-    constexpr int AHEAD = 4; // rows under way at once
-    for (int base = group; base < M; base += AHEAD * GROUPS)
-    {
-        typename L::Raw rx[AHEAD], rgy[AHEAD];
-        float mean[AHEAD], rstd[AHEAD];
-#pragma unroll
-        for (int u = 0; u < AHEAD; u++)
+        for (int k = 0; k < G; k++)
+            aw[k] = ab[k] = 0.0f;
+        constexpr int AHEAD = 4; // rows under way at once
+        for (int base = group; base < M; base += AHEAD * GROUPS)
         {
-            const int row = base + u * GROUPS < M ? base + u * GROUPS : M - 1;
-            const int64_t at = (int64_t)row * N + c;
-            if (!TINY)
-            {
-                rx[u] = L::load_raw(x + at);
-                rgy[u] = L::load_raw(gy + at);
-            }
-            else
-            {
-                float v[G];
-                L::load(x + at, 0, N, 0.0f, v);
-                rx[u] = L::pack(v);
-                L::load(gy + at, 0, N, 0.0f, v);
-                rgy[u] = L::pack(v);
-            }
-            mean[u] = mean_in[row];
-            rstd[u] = rstd_in[row];
-        }
+            typename L::Raw rx[AHEAD], rgy[AHEAD];
+            float mean[AHEAD], rstd[AHEAD];
 #pragma unroll
-        for (int u = 0; u < AHEAD; u++)
-        {
-            float xv[G], gv[G];
-            L::unpack(rx[u], xv);
-            L::unpack(rgy[u], gv);
-            if (base + u * GROUPS < M)
+            for (int u = 0; u < AHEAD; u++)
             {
-#pragma unroll
-                for (int k = 0; k < G; k++)
+                const int row = base + u * GROUPS < M ? base + u * GROUPS : M - 1;
+                const int64_t at = (int64_t)row * N + c;
+                if (!TINY)
                 {
-                    aw[k] = aw[k] + gv[k] * ((xv[k] - mean[u]) * rstd[u]);
-                    ab[k] = ab[k] + gv[k];
+                    rx[u] = L::load_raw(x + at);
+                    rgy[u] = L::load_raw(gy + at);
+                }
+                else
+                {
+                    float v[G];
+                    L::load(x + at, 0, N, 0.0f, v);
+                    rx[u] = L::pack(v);
+                    L::load(gy + at, 0, N, 0.0f, v);
+                    rgy[u] = L::pack(v);
+                }
+                mean[u] = mean_in[row];
+                rstd[u] = rstd_in[row];
+            }
+#pragma unroll
+            for (int u = 0; u < AHEAD; u++)
+            {
+                float xv[G], gv[G];
+                L::unpack(rx[u], xv);
+                L::unpack(rgy[u], gv);
+                found = found || ln_offset_saved(mean[u], rstd[u]);
+                if (base + u * GROUPS < M)
+                {
+#pragma unroll
+                    for (int k = 0; k < G; k++)
+                    {
+                        const float d = REST ? (xv[k] - mean[u]) - rest[base + u * GROUPS] : xv[k] - mean[u];
+                        aw[k] = aw[k] + gv[k] * (d * rstd[u]);
+                        ab[k] = ab[k] + gv[k];
+                    }
                 }
             }
         }
+    };
+    if (tid == 0)
+        some = 0;
+    lds_barrier();
+    accumulate(std::false_type());
+    if (found)
+        some = 1;
+    lds_barrier();
+    if (some) // offset rows: what their means leave, a wave a row (a lane's granules in turn, a butterfly), and the sums again
+    {
+        constexpr int WAVES = THREADS / 64;
+        static_assert(64 * WAVES >= LN_FEW_ROWS, "a lane for every row");
+        const int wave = __builtin_amdgcn_readfirstlane(tid / 64), at = tid % 64, mine = wave + WAVES * at;
+        const float mean = mine < M ? mean_in[mine] : 0.0f;
+        const bool offset = mine < M && ln_offset_saved(mean, rstd_in[mine]);
+        if (mine < M && !offset)
+            rest[mine] = 0.0f;
+        for (uint64_t left = __ballot(offset); left != 0; left &= left - 1)
+        {
+            const int from = __builtin_ctzll(left), row = wave + WAVES * from;
+            const float m = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mean), from));
+            const typename L::T *xr = x + (int64_t)row * N;
+            float t = 0.0f, v[G];
+            int c = at * G;
+            constexpr int AHEAD = 8;
+            for (int to = AHEAD * 64 * G; to <= N; to += AHEAD * 64 * G, c += AHEAD * 64 * G) // whole rounds of the wave
+            {
+                typename L::Raw raw[AHEAD];
+#pragma unroll
+                for (int u = 0; u < AHEAD; u++)
+                    raw[u] = L::load_raw(xr + c + u * 64 * G);
+#pragma unroll
+                for (int u = 0; u < AHEAD; u++)
+                {
+                    L::unpack(raw[u], v);
+#pragma unroll
+                    for (int k = 0; k < G; k++)
+                        v[k] = v[k] - m;
+                    t = t + granule_sum<G>(v);
+                }
+            }
+            for (; c < N; c += 64 * G)
+            {
+                L::load(xr, c, N, m, v);
+#pragma unroll
+                for (int k = 0; k < G; k++)
+                    v[k] = v[k] - m;
+                t = t + granule_sum<G>(v);
+            }
+            t = lanes_sum<64>(t);
+            if (at == 0)
+                rest[row] = t * inv_n;
+        }
+        lds_barrier();
+        accumulate(std::true_type());
     }
 #pragma unroll
     for (int which = 0; which < 2; which++)
@@ -678,20 +876,40 @@ __global__ __launch_bounds__(ln_grad_threads(TPR)) void layer_norm_grad_few_kern
     }
 }
 
-// The same for rows too long for the registers: gx by a workgroup per row that reads it twice ...
+// The same for rows too long for the registers: gx by a workgroup per row that reads it twice (an offset row three times), and what the
+// row's mean leaves ...
 template <int DT, int PDT>
 __global__ __launch_bounds__(1024) void layer_norm_grad_long_kernel(
     const typename LowpType<DT>::T *__restrict__ gy, const typename LowpType<DT>::T *__restrict__ x,
     const typename LowpType<PDT>::T *__restrict__ w, const float *__restrict__ mean_in, const float *__restrict__ rstd_in,
-    typename LowpType<DT>::T *__restrict__ gx, int64_t N, float inv_n)
+    typename LowpType<DT>::T *__restrict__ gx, float *__restrict__ rest_out, int64_t N, float inv_n)
 {
     typedef Lowp<DT> L;
     constexpr int G = L::G, TPR = 1024;
-    __shared__ float scratch[2 * (TPR / 64)];
+    __shared__ float scratch[2 * (TPR / 64)], rest_scratch[TPR / 64];
     const int j = threadIdx.x;
     const int64_t row = blockIdx.x;
     const float mean = mean_in[row], rstd = rstd_in[row];
     float xv[G], gv[G], wv[G];
+    float rest = 0.0f;
+    if (ln_offset_saved(mean, rstd)) // (the whole workgroup's)
+    {
+        float t[1] = {0.0f};
+        for (int64_t c = (int64_t)j * G; c < N; c += TPR * G)
+        {
+            L::load(x + row * N, c, N, mean, xv);
+#pragma unroll
+            for (int k = 0; k < G; k++)
+                xv[k] = xv[k] - mean;
+            t[0] = t[0] + granule_sum<G>(xv);
+        }
+        team_sum<TPR, 1>(t, rest_scratch, j);
+        rest = t[0] * inv_n;
+    }
+    if (rest_out != nullptr && j == 0)
+        rest_out[row] = rest;
+    if (gx == nullptr)
+        return;
     float s[2] = {0.0f, 0.0f};
     for (int64_t c = (int64_t)j * G; c < N; c += TPR * G)
     {
@@ -701,7 +919,7 @@ __global__ __launch_bounds__(1024) void layer_norm_grad_long_kernel(
 #pragma unroll
         for (int k = 0; k < G; k++)
         {
-            const float xh = c + k < N ? (xv[k] - mean) * rstd : 0.0f;
+            const float xh = c + k < N ? ((xv[k] - mean) - rest) * rstd : 0.0f;
             if (w != nullptr)
                 gv[k] = gv[k] * wv[k];
             xv[k] = gv[k] * xh;
@@ -719,7 +937,7 @@ __global__ __launch_bounds__(1024) void layer_norm_grad_long_kernel(
 #pragma unroll
         for (int k = 0; k < G; k++)
         {
-            const float xh = (xv[k] - mean) * rstd;
+            const float xh = ((xv[k] - mean) - rest) * rstd;
             if (w != nullptr)
                 gv[k] = gv[k] * wv[k];
             gv[k] = rstd * ((gv[k] - m1) - xh * m2);
@@ -733,7 +951,8 @@ template <int DT>
 __global__ __launch_bounds__(256) void layer_norm_param_long_kernel(const typename LowpType<DT>::T *__restrict__ gy,
                                                                     const typename LowpType<DT>::T *__restrict__ x,
                                                                     const float *__restrict__ mean_in,
-                                                                    const float *__restrict__ rstd_in, float *__restrict__ partial,
+                                                                    const float *__restrict__ rstd_in,
+                                                                    const float *__restrict__ rest_in, float *__restrict__ partial,
                                                                     int64_t M, int64_t N, int64_t rows_per_block)
 {
     typedef Lowp<DT> L;
@@ -752,11 +971,11 @@ __global__ __launch_bounds__(256) void layer_norm_param_long_kernel(const typena
         float xv[G], gv[G];
         L::load(x + row * N, c, N, 0.0f, xv);
         L::load(gy + row * N, c, N, 0.0f, gv);
-        const float mean = mean_in[row], rstd = rstd_in[row];
+        const float mean = mean_in[row], rstd = rstd_in[row], rest = rest_in[row];
 #pragma unroll
         for (int k = 0; k < G; k++)
         {
-            aw[k] = aw[k] + gv[k] * ((xv[k] - mean) * rstd);
+            aw[k] = aw[k] + gv[k] * (((xv[k] - mean) - rest) * rstd);
             ab[k] = ab[k] + gv[k];
         }
     }
@@ -888,10 +1107,11 @@ int64_t ln_rows_per_block(int64_t M, int64_t N, int dtype)
     return repdl_cdiv(rows < 4 ? 4 : rows, teams) * teams;
 }
 
+int64_t ln_partial_floats(int64_t M, int64_t N, int dtype) { return repdl_cdiv(M, ln_rows_per_block(M, N, dtype)) * 2 * N; }
+
 // Rows up to which one launch makes all gradients (layer_norm_grad_few_kernel).  Both sides, two launches against one: 64 x 1024 f32
 // 0.0081 / 0.0054 ms, 256 x 1024 0.0081 / 0.0058, 256 x 8192 0.0167 / 0.0090, 256 x 4096 bf16 0.0109 / 0.0076; 512 x 1024 f32 0.0081 / 0.0089,
 // 1024 x 4096 bf16 0.0177 / 0.0244.
-constexpr int64_t LN_FEW_ROWS = 256;
 bool ln_few_rows(int64_t M, int64_t N) { return M <= LN_FEW_ROWS && N <= LN_MAX_ONCHIP; }
 
 template <int DT, int PDT, int TPR, int E, bool TINY>
@@ -930,10 +1150,12 @@ int layer_norm_grad_typed(const void *gy, const void *x, const void *w, const fl
     typedef typename LowpType<PDT>::T P;
     if (N > LN_MAX_ONCHIP)
     {
-        const int rc = gx == nullptr ? REPDL_OK : repdl_launch_slices(M, 1024, [&](int64_t row, unsigned count) {
+        float *rest = partial == nullptr ? nullptr : partial + ln_partial_floats(M, N, DT); // (behind the partial sums)
+        const int rc = repdl_launch_slices(M, 1024, [&](int64_t row, unsigned count) {
             REPDL_LAUNCH((layer_norm_grad_long_kernel<DT, PDT>), dim3(count), dim3(1024), 0, s, static_cast<const T *>(gy) + row * N,
                          static_cast<const T *>(x) + row * N, static_cast<const P *>(w), mean + row, rstd + row,
-                         static_cast<T *>(gx) + row * N, N, (float)(1.0 / (double)N));
+                         gx == nullptr ? nullptr : static_cast<T *>(gx) + row * N, rest == nullptr ? nullptr : rest + row, N,
+                         (float)(1.0 / (double)N));
         });
         if (rc != REPDL_OK)
             return rc;
@@ -942,7 +1164,7 @@ int layer_norm_grad_typed(const void *gy, const void *x, const void *w, const fl
             const int64_t rpb = ln_rows_per_block(M, N, DT);
             REPDL_LAUNCH((layer_norm_param_long_kernel<DT>),
                          dim3((unsigned)repdl_cdiv(N, 256 * Lowp<DT>::G), (unsigned)repdl_cdiv(M, rpb)), dim3(256), 0, s,
-                         static_cast<const T *>(gy), static_cast<const T *>(x), mean, rstd, partial, M, N, rpb);
+                         static_cast<const T *>(gy), static_cast<const T *>(x), mean, rstd, rest, partial, M, N, rpb);
         }
         return repdl_launch_status();
     }
@@ -1011,7 +1233,7 @@ REPDL_API int repdl_hip_layer_norm_grad(const void *grad_y, const void *x, const
     if (params && M > 0 && !one_launch)
     {
         hipError_t e = repdl_ws_acquire(reinterpret_cast<void **>(&partial),
-                                        (size_t)repdl_cdiv(M, ln_rows_per_block(M, N, dtype)) * 2 * (size_t)N * sizeof(float), s);
+                                        (size_t)(ln_partial_floats(M, N, dtype) + (N > LN_MAX_ONCHIP ? M : 0)) * sizeof(float), s);
         if (e != hipSuccess)
             return (int)e;
     }
