@@ -59,6 +59,7 @@ __global__ __launch_bounds__(256) void preference_rows_kernel(const typename Low
 {
     typedef Lowp<DT> L;
     constexpr int G = L::G, GPT = E / G, TEAMS = 256 / TPR;
+    constexpr int DEGREE = DT == REPDL_F32 ? 6 : 5; // of the terms' polynomial
     __shared__ float wave_m[4], wave_s[4];
     const int tid = threadIdx.x, j = tid % TPR;
     if (p.first + blockIdx.x == 0 && tid == 0)
@@ -136,7 +137,7 @@ __global__ __launch_bounds__(256) void preference_rows_kernel(const typename Low
             float e[G];
 #pragma unroll
             for (int k = 0; k < G; k++)
-                e[k] = crm_exp_term(__builtin_amdgcn_fmed3f(v[i][k], least, top), shift, DT == REPDL_F32 ? 6 : 5);
+                e[k] = crm_exp_term(__builtin_amdgcn_fmed3f(v[i][k], least, top), shift, DEGREE);
 #pragma unroll
             for (int step = 1; step < G; step <<= 1)
 #pragma unroll
@@ -154,7 +155,17 @@ __global__ __launch_bounds__(256) void preference_rows_kernel(const typename Low
         s = ((wave_s[0] + wave_s[1]) + wave_s[2]) + wave_s[3];
     }
     if (j == 0)
-        part[(int64_t)row * p.chunks + chunk] = make_float2(m, s * crm_exp_base(top, shift));
+    {
+        const float base = crm_exp_base(top, shift);
+        float sum = s * base;
+        // A row that one token owns: the maximum's own term times the base is 1 but for the polynomial's error of up to 4.9e-7, so the
+        // token's log probability would come out as that, of either sign, instead of 0, and 1 - p in the gradient likewise.  Below 1 + 2^-16
+        // (thirty times the error: no such row is missed) that term counts as exactly 1.  s is at least it: rounded sums of positive
+        // terms do not fall below one of them.  (A vocabulary of a single token keeps its one term as the sum has it.)
+        if (sum > 0.5f && sum < 1.0f + 0x1p-16f && p.vocab > 1)
+            sum = 1.0f + (s - crm_exp_term(top, shift, DEGREE)) * base;
+        part[(int64_t)row * p.chunks + chunk] = make_float2(m, sum);
+    }
 }
 
 constexpr int PAIR_THREADS = 1024;
@@ -246,7 +257,7 @@ __global__ __launch_bounds__(PAIR_THREADS) void preference_pairs_kernel(const in
             lds_barrier(); // (the tables)
         if (live && t != p.ignore)
         {
-            // s >= 1 - 2^-20 (the maximum's own term is 1 but for the polynomial's error) unless the row holds a NaN, +inf or nothing but -inf
+            // s >= 1 (a single token's vocabulary: 1 - 2^-20) unless the row holds a NaN, +inf or nothing but -inf
             const double lp = s > 0.5f ? ((double)x - (double)m) - crm_log64_core((double)s, tables.log_tables()) : __builtin_nan("");
             acc = acc + lp;
             if (row_stats != nullptr)
