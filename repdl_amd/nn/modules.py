@@ -63,11 +63,13 @@ class LayerNorm(torch.nn.LayerNorm):
 class Dropout(torch.nn.Dropout):
     """Dropout whose masks are a function of the layer's seed and of how often it has been called, on any device.
 
-    ``rng_state`` (int64: seed, number of the next call) is a buffer that moves with the module and, like everything of
-    ``torch.nn.Dropout``, is not part of the state_dict: save it beside the weights to go on with the masks of an
-    interrupted run.  ``seed`` (in [0, 2^63)) defaults to a draw from PyTorch's CPU generator.  A layer that is copied
-    (``copy.deepcopy``) draws the same masks as its original: give copies that are to differ a seed of their own.  The call
-    number goes up on the device: calls of one layer on several streams at once need an order between them.
+    ``rng_state`` (int64: seed, number of the next call) moves with the module and, like everything of ``torch.nn.Dropout``,
+    is not part of the state_dict: save it beside the weights to go on with the masks of an interrupted run.  It is no
+    buffer: what keeps buffers alike over the ranks of a data-parallel run (DistributedDataParallel's default) would give
+    every rank the masks of the first.  Ranks that are to differ take seeds of their own.
+    ``seed`` (in [0, 2^63)) defaults to a draw from PyTorch's CPU generator.  A layer that is copied (``copy.deepcopy``)
+    draws the same masks as its original: give copies that are to differ a seed of their own.  The call number goes up on
+    the device: calls of one layer on several streams at once need an order between them.
     Recomputing a forward pass (activation checkpointing) takes another call and so another mask: use
     ``functional.dropout`` with the state of the first one there.
     ``forward(input, residual)`` adds the residual in the same pass."""
@@ -80,7 +82,12 @@ class Dropout(torch.nn.Dropout):
             seed = int(torch.randint(0, 2 ** 63 - 1, (), dtype=torch.int64))
         if not 0 <= seed < 2 ** 63:
             raise ValueError("Dropout: the seed is an integer in [0, 2^63)")
-        self.register_buffer("rng_state", torch.tensor([seed, 0], dtype=torch.int64), persistent=False)
+        self.rng_state = torch.tensor([seed, 0], dtype=torch.int64)
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        self.rng_state = fn(self.rng_state)
+        return self
 
     def forward(self, input: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         if not self.training or self.p == 0.0:
