@@ -79,7 +79,7 @@ class Dropout(torch.nn.Dropout):
         if inplace:
             raise NotImplementedError("Dropout: in-place is not supported")
         if seed is None:
-            seed = int(torch.randint(0, 2 ** 63 - 1, (), dtype=torch.int64))
+            seed = int(torch.randint(0, 2 ** 63 - 1, (), dtype=torch.int64, device="cpu"))
         if not 0 <= seed < 2 ** 63:
             raise ValueError("Dropout: the seed is an integer in [0, 2^63)")
         self.rng_state = torch.tensor([seed, 0], dtype=torch.int64)

@@ -38,3 +38,13 @@ def test_what_a_module_does_with_it():
     for move in (net.half, net.double, net.bfloat16, net.cpu, lambda: net.to("cpu", torch.float16)):
         assert move()[0].rng_state.tolist() == [9, 4] and net[0].rng_state.dtype == torch.int64
     assert net.to("meta")[0].rng_state.device.type == "meta"  # it goes where the module goes
+
+
+def test_the_seed_is_drawn_on_the_cpu():
+    """Also where a default device is set, whose generator -- and whose values, if it has any -- would be another's."""
+    torch.manual_seed(3)
+    want = [nn.Dropout(0.5).rng_state.tolist() for _ in range(2)]
+    torch.manual_seed(3)
+    with torch.device("meta"):
+        assert nn.Dropout(0.5).rng_state.is_meta
+    assert nn.Dropout(0.5).rng_state.tolist() == want[1]
