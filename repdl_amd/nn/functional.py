@@ -302,7 +302,11 @@ def dropout(input: torch.Tensor, p: float, state: Union[torch.Tensor, Tuple[int,
     if not 0.0 <= p <= 1.0:
         raise ValueError("dropout probability has to be between 0 and 1, but got %s" % p)
     if not training or p == 0.0:
-        return input if residual is None else residual + input
+        if residual is None:
+            return input
+        if residual.shape != input.shape or residual.dtype != input.dtype:  # (as in training)
+            raise RuntimeError("residual and input differ in shape or type")
+        return residual + input
     if not _needs_grad(input, residual):
         return ops.dropout(input, p, state, residual)
     return ops._backend(input).dropout_autograd(input, residual, float(p), *ops._dropout_state(state))
