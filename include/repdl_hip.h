@@ -352,7 +352,7 @@ int repdl_hip_dropout_next_call(int64_t *state, int64_t *used, void *stream);
  *   loss[0]  = mean over pairs of (1 - label_smoothing) * softplus(-z_p) + label_smoothing * softplus(z_p)
  *   logps[i] = L_i, [2 * pairs]
  * row_stats [2 * pairs, steps, 2] (8-byte aligned) and coef [2 * pairs] are what the backward pass takes (both NULL: not
- * wanted).  A target outside [0, vocab) that is not ignore_index, a NaN or +inf logit and a row of nothing but -inf make their
+ * wanted; one without the other is refused).  A target outside [0, vocab) that is not ignore_index, a NaN or +inf logit and a row of nothing but -inf make their
  * sequence's log probability, the loss and the pair's gradient NaN; a target whose logit is -inf makes its sequence's log
  * probability -inf (and the loss +inf, where that is the preferred answer).
  * preference_loss_grad: grad_logits [2 * pairs, steps, vocab], contiguous, = grad_loss[0] (device memory) * d loss / d logits;

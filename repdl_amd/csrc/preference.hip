@@ -499,6 +499,7 @@ REPDL_API int repdl_hip_preference_loss(const void *logits, const int64_t *targe
 {
     REPDL_REQUIRE(pref_shape_ok(pairs, steps, vocab, seq_stride, step_stride, dtype));
     REPDL_REQUIRE(loss != nullptr && logps != nullptr && (steps == 0 || (logits != nullptr && target != nullptr)));
+    REPDL_REQUIRE((row_stats != nullptr) == (coef != nullptr) || (steps == 0 && coef != nullptr)); // (no rows: no statistics)
     hipStream_t s = repdl_stream(stream);
     PrefShape p = pref_shape(pairs, steps, vocab, seq_stride, step_stride, ignore_index, PREF_CHUNK);
     // scratch: (m, sum) per row and chunk, the pairs' losses, the target's logit per row, a counter
