@@ -320,10 +320,9 @@ CRM_FN float crm_log_wide(float x, crm_log_tables_wide tab)
 
 // ---- exp of a difference to the row's maximum, in binary32 ---------------------------------------
 // exp(d) for d <= 0 as 2^n 2^f with n + f = d log2(e): one multiplication, a rounding to the nearest integer, a polynomial
-// of degree 6 in f (|f| <= 1/2; minimax in the relative error, coefficients rounded to binary32: 2.2e-8) in single-rounding
-// fused multiply-adds, and a scaling by 2^n.  13 binary32 instructions against 29 mostly binary64 ones of crm_exp: for the
+// of degree 6 in f (|f| <= 1/2) in single-rounding fused multiply-adds, and a scaling by 2^n.  13 binary32 instructions against 29 mostly binary64 ones of crm_exp: for the
 // losses over large vocabularies, whose row sums hold it to a few 2^-24 anyway.  Relative error at most 2^-23 + 1.25 |d| 2^-24:
-// the polynomial in binary32 8.2e-8, the rounded product |d log2(e)| 2^-24 ln 2 = |d| 2^-24, and binary32's log2(e), which is
+// the polynomial in binary32 7.9e-8, the rounded product |d log2(e)| 2^-24 ln 2 = |d| 2^-24, and binary32's log2(e), which is
 // 1.335e-8 = 0.224 * 2^-24 below log2(e), relative, and so another 0.224 |d| 2^-24.
 // -inf gives +0 (so does every d below -105: the result rounds to 0); NaN gives +0, so callers carry a NaN by other means.
 #if CRM_DEVICE
@@ -338,52 +337,50 @@ CRM_FN float crm_ldexpf(float a, int e) { return ldexpf(a, e); }
 CRM_FN float crm_fmaxf(float a, float b) { return fmaxf(a, b); }
 #endif
 
+// 2^f for |f| <= 1/2, degree 5 or 6 (coefficients and the polynomials' own errors, 1.08e-7 and 1.59e-8: crmath_tables.h); exactly 1 at 0
+CRM_FN float crm_exp2_poly(float f, int degree)
+{
+    float p;
+    if (degree == 5)
+    {
+        p = CRM_EXP2_5_C5;
+        p = crm_fmaf(p, f, CRM_EXP2_5_C4);
+        p = crm_fmaf(p, f, CRM_EXP2_5_C3);
+        p = crm_fmaf(p, f, CRM_EXP2_5_C2);
+        p = crm_fmaf(p, f, CRM_EXP2_5_C1);
+    }
+    else
+    {
+        p = CRM_EXP2_6_C6;
+        p = crm_fmaf(p, f, CRM_EXP2_6_C5);
+        p = crm_fmaf(p, f, CRM_EXP2_6_C4);
+        p = crm_fmaf(p, f, CRM_EXP2_6_C3);
+        p = crm_fmaf(p, f, CRM_EXP2_6_C2);
+        p = crm_fmaf(p, f, CRM_EXP2_6_C1);
+    }
+    return crm_fmaf(p, f, 1.0f);
+}
+
 CRM_FN float crm_exp_neg(float d)
 {
     const float y = crm_fmaxf(d * 0x1.715476p+0f, -160.0f);
     const float n = crm_rintf(y);
     const float f = y - n; // exact
-    float p = 0x1.470b4ap-13f;
-    p = crm_fmaf(p, f, 0x1.5f7276p-10f);
-    p = crm_fmaf(p, f, 0x1.3b270ep-7f);
-    p = crm_fmaf(p, f, 0x1.c6ae72p-5f);
-    p = crm_fmaf(p, f, 0x1.ebfbe2p-3f);
-    p = crm_fmaf(p, f, 0x1.62e432p-1f);
-    p = crm_fmaf(p, f, 1.0f);
-    return crm_ldexpf(p, (int)n);
+    return crm_ldexpf(crm_exp2_poly(f, 6), (int)n);
 }
 
 // One term of a row's sum of exponentials, without subtracting the row's maximum m first: 2^(x L - K) for L = binary32's log2(e)
 // and the integer K = rint(m L), |K| <= 2^22.  With c = 1.5 * 2^23 - K (exact), t = fma(x, L, c) has rint(x L) - K in its low bits and
 // t - c = rint(x L); f = x L - rint(x L) comes from one fused operation; the power of two is added to the exponent field of the
 // polynomial.  The caller clamps x to at least m - 86, so that no exponent field falls below 1 (what lies below is worth less than 2^-124 of
-// the maximum's term).  sum * crm_exp_base(m, K) is the sum of exp(x - m).  Degree 6 as above; degree 5 (4.9e-7 with its
-// coefficients and steps in binary32) is one instruction less where 16-bit logits make the sum bound by the vector ALU.
-// Relative error of a term: 2^-23 (5: 2^-21) + 0.224 |x - m| 2^-24 -- the product x L is not rounded.
+// the maximum's term).  sum * crm_exp_base(m, K) is the sum of exp(x - m).  Degree 6 as above; degree 5 (1.7e-7 with its
+// coefficients and steps in binary32, against 0.8e-7) is one instruction less where 16-bit logits make the sum bound by the vector ALU.
+// Relative error of a term: 2^-23 (5: 2^-22) + 0.224 |x - m| 2^-24 -- the product x L is not rounded.
 CRM_FN float crm_exp_term(float x, float c, int degree)
 {
     const float t = crm_fmaf(x, 0x1.715476p+0f, c);
     const float f = crm_fmaf(x, 0x1.715476p+0f, -(t - c));
-    float p;
-    if (degree == 5)
-    {
-        p = 0x1.23a604p-10f;
-        p = crm_fmaf(p, f, 0x1.3cbea8p-7f);
-        p = crm_fmaf(p, f, 0x1.c74322p-5f);
-        p = crm_fmaf(p, f, 0x1.ebfa4ep-3f);
-        p = crm_fmaf(p, f, 0x1.62e39ep-1f);
-    }
-    else
-    {
-        p = 0x1.470b4ap-13f;
-        p = crm_fmaf(p, f, 0x1.5f7276p-10f);
-        p = crm_fmaf(p, f, 0x1.3b270ep-7f);
-        p = crm_fmaf(p, f, 0x1.c6ae72p-5f);
-        p = crm_fmaf(p, f, 0x1.ebfbe2p-3f);
-        p = crm_fmaf(p, f, 0x1.62e432p-1f);
-    }
-    p = crm_fmaf(p, f, 1.0f);
-    return crm_u2f((crm_f2u(t) << 23) + crm_f2u(p));
+    return crm_u2f((crm_f2u(t) << 23) + crm_f2u(crm_exp2_poly(f, degree)));
 }
 
 // K and c of crm_exp_term for a maximum of at most 2^21 in magnitude, and the factor 2^(K - m L), |K - m L| <= 1/2
@@ -391,11 +388,5 @@ CRM_FN float crm_exp_shift(float m) { return 0x1.8p23f - crm_rintf(m * 0x1.71547
 CRM_FN float crm_exp_base(float m, float c)
 {
     const float g = crm_fmaf(m, 0x1.715476p+0f, c - 0x1.8p23f); // m L - K, rounded once; 2^-g by the term's own polynomial
-    float p = 0x1.470b4ap-13f;
-    p = crm_fmaf(p, -g, 0x1.5f7276p-10f);
-    p = crm_fmaf(p, -g, 0x1.3b270ep-7f);
-    p = crm_fmaf(p, -g, 0x1.c6ae72p-5f);
-    p = crm_fmaf(p, -g, 0x1.ebfbe2p-3f);
-    p = crm_fmaf(p, -g, 0x1.62e432p-1f);
-    return crm_fmaf(p, -g, 1.0f);
+    return crm_exp2_poly(-g, 6);
 }

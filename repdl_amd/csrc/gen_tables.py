@@ -20,6 +20,9 @@ width 2^-7 above).  For interval i with centre c:
     logc_hi  = -log(invc) rounded to a multiple of 2^-43 (k*LN2_HI + logc_hi is
                then exact in binary64);
     logc_lo  = RN32(-log(invc) - logc_hi)  (below 2^-44, so binary32 keeps it to 2^-68).
+
+polynomials for 2^f in binary32, |f| <= 1/2, of degree 5 and 6 (crm_exp_neg, crm_exp_term): minimax in the relative error
+among those that are exactly 1 at f = 0, coefficients rounded to binary32.
 """
 from __future__ import annotations
 
@@ -83,6 +86,41 @@ def log_table():
     return rows
 
 
+def exp2_poly(degree: int):
+    """Coefficients c_1 .. c_degree of the polynomial 1 + c_1 f + ... whose largest relative error against 2^f, |f| <= 1/2, is least,
+    rounded to binary32, and the error then.  Remez's exchange: e(f) = 2^-f (1 + c_1 f + ...) - 1 is f times a weighted polynomial, so
+    at the best coefficients e(f) / f takes the bound of e with alternating signs at degree + 1 points; each step solves for
+    coefficients and bound at the points it has, then moves them to where |e| is largest in each run of one sign of e(f) / f."""
+    grid = [mp.mpf(i) / 4000 for i in range(-2000, 2001) if i != 0]
+    points = [mp.cos(mp.pi * (2 * i + 1) / (2 * degree + 2)) / 2 for i in reversed(range(degree + 1))]
+    points = [f if abs(f) > 0.01 else mp.mpf("0.05") for f in points]
+
+    def error(c, f):
+        return mp.mpf(2) ** -f * mp.polyval(c[::-1] + [1], f) - 1
+
+    for _ in range(30):
+        rows, right = mp.matrix(degree + 1, degree + 1), mp.matrix(degree + 1, 1)
+        for i, f in enumerate(points):
+            for j in range(degree):
+                rows[i, j] = mp.mpf(2) ** -f * f ** (j + 1)
+            rows[i, degree] = (-1) ** i * (-1 if f < 0 else 1)
+            right[i] = 1 - mp.mpf(2) ** -f
+        solution = list(mp.lu_solve(rows, right))
+        runs = []
+        for f in grid:
+            e = error(solution[:degree], f)
+            if not runs or (runs[-1][1] * runs[-1][0] > 0) != (e * f > 0):
+                runs.append((f, e))
+            elif abs(e) > abs(runs[-1][1]):
+                runs[-1] = (f, e)
+        assert len(runs) == degree + 1
+        points = [f for f, _ in runs]
+        if max(abs(e) for _, e in runs) <= abs(solution[degree]) * (1 + mp.mpf(10) ** -4):
+            break
+    rounded = [round_to_bits(c, 24) for c in solution[:degree]]
+    return [rn(c) for c in rounded], max(abs(error(rounded, f)) for f in grid)
+
+
 def main() -> None:
     ln2 = mp.log(2)
     ln2_hi = mp.nint(mp.ldexp(ln2, 43)) / mp.mpf(2) ** 43
@@ -104,6 +142,11 @@ def main() -> None:
         for i in range(0, 128, 4):
             out.append("    " + ", ".join(float.hex(r[col]) + suffix for r in rows[i:i + 4]) + ", \\")
         out.append("}")
+    for degree in (5, 6):
+        coefficients, error = exp2_poly(degree)
+        out.append("// 2^f, |f| <= 1/2: 1 + C1 f + ... of degree %d, relative error %s" % (degree, mp.nstr(error, 3)))
+        for i, c in enumerate(coefficients):
+            out.append("#define CRM_EXP2_%d_C%d %sf" % (degree, i + 1, float.hex(c)))
     with open(os.path.join(HERE, "crmath_tables.h"), "w") as f:
         f.write("\n".join(out) + "\n")
 

@@ -158,9 +158,9 @@ __global__ __launch_bounds__(256) void preference_rows_kernel(const typename Low
     {
         const float base = crm_exp_base(top, shift);
         float sum = s * base;
-        // A row that one token owns: the maximum's own term times the base is 1 but for the polynomial's error of up to 4.9e-7, so the
+        // A row that one token owns: the maximum's own term times the base is 1 but for an error of up to 2.2e-7 (degree 6: 1.2e-7), so the
         // token's log probability would come out as that, of either sign, instead of 0, and 1 - p in the gradient likewise.  Below 1 + 2^-16
-        // (thirty times the error: no such row is missed) that term counts as exactly 1.  s is at least it: rounded sums of positive
+        // (seventy times the error: no such row is missed) that term counts as exactly 1.  s is at least it: rounded sums of positive
         // terms do not fall below one of them.  (A vocabulary of a single token keeps its one term as the sum has it.)
         if (sum > 0.5f && sum < 1.0f + 0x1p-16f && p.vocab > 1)
             sum = 1.0f + (s - crm_exp_term(top, shift, DEGREE)) * base;
@@ -257,7 +257,7 @@ __global__ __launch_bounds__(PAIR_THREADS) void preference_pairs_kernel(const in
             lds_barrier(); // (the tables)
         if (live && t != p.ignore)
         {
-            // s >= 1 (a single token's vocabulary: 1 - 2^-20) unless the row holds a NaN, +inf or nothing but -inf
+            // s >= 1 (a single token's vocabulary: 1 - 2^-22) unless the row holds a NaN, +inf or nothing but -inf
             const double lp = s > 0.5f ? ((double)x - (double)m) - crm_log64_core((double)s, tables.log_tables()) : __builtin_nan("");
             acc = acc + lp;
             if (row_stats != nullptr)
