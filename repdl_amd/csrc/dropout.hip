@@ -13,8 +13,8 @@
 //
 // Bound: HBM, 8 B per element in binary32 (12 with a residual), 4 (6) in 16 bits.  The ten rounds are 20 products of 32 by 32
 // to 64 bits (a quarter of the vector rate each) and about 20 three-operand exclusive ors for four elements, 25 issue slots per
-// element: 39.3e12 / 25 = 1.6e12 elements/s, which at 16 bits is 6.3 TB/s, just above the copy rate.  Measured (a copy of 1 GiB moves 5.1 TB/s):
-// 2^26 f32 0.086 ms = 6.2 TB/s, with a residual 0.125 = 6.4; 2^27 bf16 0.092 = 5.9, with a residual 0.134 = 6.0; 64000 f32 3.1 us.
+// element: 39.3e12 / 25 = 1.6e12 elements/s, which at 16 bits is 6.3 TB/s, what a copy reaches.  Measured (a non-temporal copy of 1 GiB moves 6.3 TB/s):
+// 2^26 f32 0.086 ms = 6.2 TB/s, with a residual 0.127 = 6.4; 2^27 bf16 0.096 = 5.6, f16 0.097, with a residual 0.135 = 6.0, 0.136; 64000 f32 2.9 us.
 #include "lowp.h"
 
 namespace
@@ -47,7 +47,9 @@ struct DropoutArgs
     float scale;
 };
 
-// A thread takes DROP_GRANULES 16-byte granules, a workgroup's span apart.
+// A thread takes DROP_GRANULES 16-byte granules, a workgroup's span apart.  One / two / four / eight, ms: 2^27 bf16 0.093 / 0.091 / 0.096 / 0.107, with a
+// residual 0.132 / 0.133 / 0.135 / 0.226; 2^26 f32 0.086 / 0.086 / 0.086 / 0.090; 2^26 bf16 0.042 / 0.043 / 0.051 / 0.050; 12345677 f32 with a residual 0.0224 / 0.0222 /
+// 0.0232 / 0.0234, bf16 0.0146 / 0.0162 / 0.0172 / 0.0204; 64000 f32 0.0024 / 0.0025 / 0.0029 / 0.0041.  Fewer would do as well or better, with the same bits.
 constexpr int DROP_THREADS = 256, DROP_GRANULES = 4;
 
 template <int DT, bool RES, bool STREAM>

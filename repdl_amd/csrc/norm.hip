@@ -24,8 +24,8 @@
 //
 // The two passes over a row (mean, then centred squares) read it from registers: one thread holds E = 16 or 24 of its elements, as
 // 16-byte granules TPR granules apart, TPR threads a row.  Bound: HBM, 2 passes over the tensor forward and 3 backward.  Measured
-// (a copy of 1 GiB moves 5.1 TB/s): forward 16384 x 8192 bf16 0.094 ms = 5.7 TB/s, 8192 x 1024 f32 0.0130 = 5.2, 65536 x 256 f32
-// 0.027 = 5.0; backward with both launches 0.166 ms = 4.8 TB/s, 0.026 = 3.8, 0.048 = 4.2.
+// (a non-temporal copy of 1 GiB moves 6.3 TB/s): forward 16384 x 8192 bf16 0.096 ms = 5.6 TB/s, 8192 x 1024 f32 0.0124 = 5.4, 65536 x 256 f32
+// 0.024 = 5.6; backward with both launches 0.170 ms = 4.7 TB/s, 0.0219 = 4.6, 0.038 = 5.3.
 #include <type_traits>
 
 #include "lowp.h"

@@ -16,8 +16,8 @@
 // Bound: HBM, and for 16-bit logits level with it the vector ALU.  A column of the forward pass is 13 instructions -- widen, half
 // a maximum, clamp, 9 of crm_exp_term, an addition -- so 39.3e12 / 13 = 3e12 columns/s are 6 TB/s of 16-bit ones.  Measured, three
 // quarters of the tokens counted: 8192 x 131072 bf16 forward 0.281 ms = 5.7 TB/s read (0.351 with the exponential as
-// crm_exp_neg of a difference, 16 instructions; degree 6 here 0.304), backward 0.660 ms = 5.7 TB/s; 8192 x 32000 f32 forward 0.120 ms =
-// 6.5, backward 0.340 = 5.4; a pair of 12 tokens x 1000 7 + 5 us.
+// crm_exp_neg of a difference, 16 instructions; degree 6 here 0.304), backward 0.670 ms = 5.6 TB/s; 8192 x 32000 f32 forward 0.120 ms =
+// 6.5, backward 0.340 = 5.4; a pair of 12 tokens x 1000 4 + 3 us, backward 4.
 //
 // The row sum is in binary32 in a fixed order (a thread's granules in turn, a butterfly over the wave, the waves, the chunks),
 // which the vocabulary and the type determine alone.  Everything per token and per pair after it is in binary64: L is a sum
@@ -403,10 +403,15 @@ __global__ __launch_bounds__(256, 4) void preference_grad_kernel(const typename 
 }
 
 // ---- host -------------------------------------------------------------------------------------
+// Vocabularies of up to 1024 and 4096 columns go to a wave, 16 or 64 columns a lane, longer ones to workgroups of up to 16384.  Both sides, ms, every
+// token counted, rows x vocabulary (f32 | bf16):
+//   16 / 64 a lane      8192 x 100   0.0106 / 0.0146 | 0.0109 / 0.0148     8192 x 1000  0.0134 / 0.0161 | 0.0113 / 0.0150     131072 x 1000  0.125 / 0.132 | 0.070 / 0.107
+//   wave / workgroup    8192 x 1100  0.0170 / 0.0414 | 0.0166 / 0.0313     8192 x 4096  0.0283 / 0.0425 | 0.0207 / 0.0317     24 x 4000      0.0077 / 0.0081 | 0.0078 / 0.0079
+//   16384 / 8192 columns a workgroup   8192 x 32000 0.164 / 0.481 | 0.101 / 0.110     8192 x 131072 bf16 0.371 / 0.439     1288 x 50257 0.0465 / 0.107 | 0.0330 / 0.0309
 constexpr int PREF_E = 64, PREF_SMALL_E = 16;
-constexpr int64_t PREF_WAVE_SMALL = 64 * PREF_SMALL_E; // vocabularies that a wave holds, 16 or 64 columns a lane
+constexpr int64_t PREF_WAVE_SMALL = 64 * PREF_SMALL_E;
 constexpr int64_t PREF_WAVE = 64 * PREF_E;
-constexpr int64_t PREF_CHUNK = 256 * PREF_E; // columns that a workgroup holds
+constexpr int64_t PREF_CHUNK = 256 * PREF_E;
 
 // Chunks of about equal width, in whole rounds of a workgroup's granules (2048 columns are one of 16-bit elements, two of binary32):
 // all rounds but a row's last are full.
@@ -466,6 +471,10 @@ int launch_pref_rows(const void *logits, const int64_t *target, float2 *part, fl
     });
 }
 
+// The gradient of up to 1024 columns by a wave, 16 a lane; against a workgroup, as above: 8192 x 100 0.0044 / 0.0102 | 0.0055 / 0.0107, 8192 x 1000 0.0119 / 0.0152 |
+// 0.0078 / 0.0121, 131072 x 1000 0.213 / 0.206 | 0.099 / 0.164.  Longer ones by workgroups of 32 columns a thread; 16 / 32 / 64: 8192 x 5000 0.0750 / 0.0612 / 0.0749 |
+// 0.0333 / 0.0295 / 0.0291, 8192 x 10000 0.113 / 0.129 / 0.127 | 0.057 / 0.067 / 0.065, 8192 x 32000 0.366 / 0.384 / 0.403 | 0.180 / 0.196 / 0.193, 8192 x 131072 bf16 0.712 / 0.721 /
+// 0.742, 1288 x 50257 0.099 / 0.100 / 0.115 | 0.042 / 0.043 / 0.047, 24 x 32000 0.0045 / 0.0054 / 0.0092 | 0.0033 / 0.0041 / 0.0061.
 constexpr int PREF_GRAD_E = 32;
 
 template <int DT>
