@@ -294,7 +294,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR, 8) void layer_norm_kernel(
         lds_barrier();
         other = offsets[TEAMS - 1 - team];
     }
-    if (ln_any<TPR>(offset, other)) // (a row that is not offset but goes along ends with the bits it had)
+    if (__builtin_expect(ln_any<TPR>(offset, other), 0)) // (a row that is not offset but goes along ends with the bits it had)
     {
         s[0] = 0.0f;
 #pragma unroll
@@ -538,7 +538,7 @@ __global__ __launch_bounds__(ln_grad_threads(TPR), TPR < 1024 ? 2 : 4) void laye
 #pragma unroll
             for (int k = 0; k < G; k++)
                 xv[i][k] = xv[i][k] - mean;
-        if (any)
+        if (__builtin_expect(any, 0)) // (out of the loop's way: 4096 x 16384 f32 0.174 -> 0.168 ms)
         {
             ln_centre_again<TPR>(rg, xv, offset, scratch[half][team], j, N, inv_n);
             half ^= 1;
